@@ -62,6 +62,11 @@ SIGNATURES = {
     "gr_pg_masking_defense": (_i, [_vp, _vp, _i, _i, _i, _i, _i, _f, _vp, _vp, _vp]),
     "gr_model_input_grad": (_i, [_vp, _vp, _vp, _i, _i, _vp, _vp, _vp]),
     "gr_tr_hits": (_i, [_vp, _vp, _vp, _i, _i, _vp, _vp, _i, _i, _i, _vp, _f, _i, _i, _i64, _i64, _vp, _vp, _vp, _vp]),
+    "gr_w4_create": (_i, [_vp, _vp, _i64, _vp, _i, _i64, _vp, _i64, _vp, _i, _i, _i, _i, _vp, C.POINTER(_vp)]),
+    "gr_w4_destroy": (None, [_vp]),
+    "gr_linear_w4": (_i, [_vp, _vp, _vp, _i, _i64, _i64, _i, _vp, _i64, _vp]),
+    "gr_linear_w4_input_grad": (_i, [_vp, _vp, _vp, _i, _i64, _i64, _vp, _i64, _vp, _i64, _vp]),
+    "gr_distill_topk": (_i, [_vp, _vp, _i, _i64, _i, _i64, _vp, _vp, _i, _i, _i64, _vp, _f, _vp, _vp, _vp, _i64, _vp]),
     "gr_wb_forward": (_i, [_vp, _vp, _vp, _vp, _i, _i, _vp, _i, _i, _vp, _vp]),
     "gr_wb_backward": (_i, [_vp, _vp, _vp, _vp, _i, _i, _vp, _i, _i, _vp, _vp, _vp]),
 }
@@ -107,10 +112,10 @@ def device_index():
     return torch.cuda.current_device()
 
 
-def ctx():
-    """One gr_ctx per device, created on first use."""
+def ctx(dev=None):
+    """One gr_ctx per device (default: the current one), created on first use."""
     lib = load_library()
-    dev = device_index()
+    dev = device_index() if dev is None else dev
     with _lock:
         c = _ctxs.get(dev)
         if c is None:
@@ -157,8 +162,27 @@ def profile_read():
             for i in range(n)}
 
 
-def _stream():
-    return _vp(torch.cuda.current_stream().cuda_stream)
+def _stream(device=None):
+    return _vp(torch.cuda.current_stream(device).cuda_stream)
+
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # GR_DT_F32, GR_DT_BF16, GR_DT_F16
+
+
+def float_rows(t, name, device=None, cols=None):
+    """Checks of an operator's 2-D floating-point argument: on a ROCm device (`device`, if given), a type the library
+    takes, elements of a row next to each other (rows may be any distance apart).  Returns (tensor, row stride)."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise GraphiteHipError(f"{name} must be a CUDA (ROCm) tensor; graphite_amd has no CPU path")
+    if device is not None and t.device != device:
+        raise GraphiteHipError(f"{name} is on {t.device}, expected {device}")
+    if t.dtype not in DTYPES:
+        raise GraphiteHipError(f"{name} has type {t.dtype}; float32, bfloat16 and float16 are supported")
+    if t.dim() != 2 or (cols is not None and t.shape[1] != cols):
+        raise GraphiteHipError(f"{name} has shape {tuple(t.shape)}, expected [rows, {'columns' if cols is None else cols}]")
+    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        t = t.contiguous()                      # transposed, reversed or broadcast views
+    return t, (t.stride(0) if t.shape[0] > 1 else max(1, t.shape[1]))
 
 
 def to_dev(a):

@@ -258,6 +258,57 @@ int gr_wb_forward(gr_ctx* ctx, const float* orig, const float* att, const float*
 int gr_wb_backward(gr_ctx* ctx, const float* orig, const float* att, const float* mask, int H, int W,
                    const gr_wb_xform* xf, int T, int net, const float* grad_out, float* grad_att, void* stream);
 
+/* ---- 4-bit linear layers (no counterpart in the reference: its classifiers are float) ----------------------------------
+ * y[n,m] = act( bias[m] + sum_k x[n,k] * (q[m,k] - z[m,k / group]) * s[m,k / group] ), the weights held as 4-bit integers
+ * with one scale (and optionally one zero point) per `group` consecutive inputs of an output.
+ * Element types of tensors: */
+#define GR_DT_F32 0
+#define GR_DT_BF16 1
+#define GR_DT_F16 2
+typedef struct gr_w4 gr_w4;
+/* Lays the weights out for the matrix units (all pointers dev; they may be freed after the call, which synchronises the
+ * stream once; the object can then be used on any stream of the context's device, by any number of calls at a time).
+ *   q       [out_features] rows of ceil(in_features / 2) bytes, ldq bytes apart: input 2j in the low, 2j+1 in the high nibble
+ *   scales  [out_features][G], G = ceil(in_features / group), of type scale_type, rows lds ELEMENTS apart; finite
+ *   zeros   [out_features][G] bytes 0..15 (the low four bits count), rows ldz bytes apart; NULL = 8 everywhere
+ *   bias    float32 [out_features] or NULL
+ *   group   a multiple of 32; the last group of a row may be short, and group may exceed in_features (one scale per row)
+ *   input_grad != 0 keeps a second, transposed copy of the 4-bit weights for gr_linear_w4_input_grad. */
+int gr_w4_create(gr_ctx* ctx, const uint8_t* q, int64_t ldq, const void* scales, int scale_type, int64_t lds, const uint8_t* zeros,
+                 int64_t ldz, const float* bias, int out_features, int in_features, int group, int input_grad, void* stream,
+                 gr_w4** out);
+void gr_w4_destroy(gr_w4* w);
+/* x [N][in_features] (rows ldx elements apart) -> y [N][out_features] (rows ldy apart), both of type dtype; relu != 0 clamps
+ * negative results to 0.  The products are exact and the sums float32; the result is rounded to dtype once.  Elements
+ * between rows are not touched.  x and y must not overlap.  No workspace, no allocation, no synchronisation: the call can be
+ * captured into a HIP graph. */
+int gr_linear_w4(gr_ctx* ctx, const gr_w4* w, const void* x, int dtype, int64_t N, int64_t ldx, int relu, void* y, int64_t ldy,
+                 void* stream);
+/* grad_x[n,k] = sum_m grad_y[n,m] * (q[m,k] - z[m,k / group]) * s[m,k / group], 0 where gate[n,k] <= 0 (gate: the rectified
+ * activation the layer read, same type as grad_x, rows ldgate apart; NULL = no gate).  The layer's own ReLU, if it had one,
+ * is the caller's to apply to grad_y.  Same promises as gr_linear_w4.  The weights are frozen: no gradient is formed for them. */
+int gr_linear_w4_input_grad(gr_ctx* ctx, const gr_w4* w, const void* grad_y, int dtype, int64_t N, int64_t ldgy, const void* gate,
+                            int64_t ldgate, void* grad_x, int64_t ldgx, void* stream);
+
+/* ---- distillation from a teacher's top logits (the whitebox loop's loss when the victim's answer is a few scores rather than
+ * a label; gr_model_input_grad's cross entropy is the other one) ---------------------------------------------------------
+ * z [N][V] (type dtype, rows ldz apart): the student's logits, q = softmax(z / tau).  The teacher names up to k classes per
+ * row: index [N][k] int64, value [N][k] (type value_type) = its logits; rows ld_top elements apart in both, ld_top == 0: one
+ * teacher row for the whole batch.  index -1 marks an empty slot; a class named twice has its probabilities added.
+ *   teacher_lse == NULL (closed): p = softmax over the row's slots of value / tau, nothing left for the other classes
+ *   teacher_lse != NULL (open):   p_j = exp(value_j / tau - lse) with the teacher's float32 logsumexp(all logits / tau) per row
+ *                                 (one element when ld_top == 0); the others share p_rest = max(0, 1 - sum p), compared as ONE
+ *                                 class with q_rest = the student's mass outside the named classes (nothing if that set is
+ *                                 empty or all its logits are -inf)
+ *   loss[n] = tau^2 * ( sum_j p_j log(p_j / q_j) + p_rest log(p_rest / q_rest) )                     float32, or NULL
+ *   grad[n,:] = grad_loss[n] * d loss[n] / d z[n,:]  (type dtype, rows ldg apart; NULL = not wanted; grad_loss NULL = 1)
+ * grad may be z itself (ldg == ldz) but must not overlap it otherwise.  A row without slots (all -1; closed: also all values -inf) has loss 0 and gradient 0.
+ * An index outside [-1, V) makes its row's loss and gradient NaN.  1 <= k <= 1024; V <= 2^20 in the open form.  No workspace, no allocation: the call can be
+ * captured into a HIP graph.  Results do not vary between runs. */
+int gr_distill_topk(gr_ctx* ctx, const void* z, int dtype, int64_t N, int V, int64_t ldz, const int64_t* index, const void* value,
+                    int value_type, int k, int64_t ld_top, const float* teacher_lse, float tau, const float* grad_loss, float* loss,
+                    void* grad, int64_t ldg, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,266 @@
+"""4-bit linear layers (gr_linear_w4, gr_linear_w4_input_grad) against float64 on the CPU.
+
+Tolerance, per output: products are exact and sums float32, so a sum of n terms is off by at most n * 2^-23 * sum |x w|
+(2^-23: the matrix unit may cut instead of round); two-piece products of the 16-bit gradients add 2^-15 * sum |gy w|, the
+float32 product gy * s 2^-24; the stored result adds half a step of its type, |y| * eps / 2 (below float16's normal range
+2^-25)."""
+import os
+import sys
+
+import numpy as np
+import pytest
+import torch
+
+sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "oracle"))
+import lowbit_reference as R                                                # noqa: E402
+from graphite_amd import _hip                                               # noqa: E402
+from graphite_amd.linear_w4 import LinearW4, dequantize, quantize           # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def _layer(m, k, group, sdt=F32, zeros=True, bias=False, seed=0, device="cuda"):
+    g = torch.Generator().manual_seed(seed)
+    q = torch.randint(0, 256, (m, (k + 1) // 2), generator=g, dtype=torch.uint8)      # an odd row's last nibble is garbage
+    groups = -(-k // group)
+    s = (torch.rand((m, groups), generator=g) * 0.02 + 0.001).to(sdt)
+    z = torch.randint(0, 16, (m, groups), generator=g, dtype=torch.uint8) if zeros else None
+    b = torch.randn(m, generator=g) if bias else None
+    w = R.weights(q.numpy(), s.double().numpy(), None if z is None else z.numpy(), group, k)
+    return LinearW4(q.to(device), s.to(device), None if z is None else z.to(device), None if b is None else b.to(device),
+                    group=group, in_features=k), w, None if b is None else b.double().numpy()
+
+
+def _tol(ref, mag, terms, dtype, extra=0.0):
+    eps = torch.finfo(dtype).eps
+    return mag * (terms * 2.0 ** -23 + extra) * 1.01 + np.abs(ref) * eps / 2 * 1.01 + (2.0 ** -25 if dtype == F16 else 1e-37)
+
+
+def _check(got, ref, tol):
+    err = np.abs(got.double().cpu().numpy() - ref)
+    assert np.isfinite(err).all()
+    assert (err <= tol).all(), f"{(err / tol).max():.3g} of the tolerance at {np.unravel_index((err / tol).argmax(), err.shape)}"
+
+
+def _check_forward(layer, w, b, x, relu):
+    y = layer.forward(x, relu=relu)
+    assert y.dtype == x.dtype and tuple(y.shape) == (x.shape[0], w.shape[0])
+    xd = x.double().cpu().numpy()
+    ref = R.linear(xd, w, b, relu)
+    mag = np.abs(xd) @ np.abs(w).T + (0 if b is None else np.abs(b))
+    _check(y, ref, _tol(ref, mag, w.shape[1] + 64, x.dtype))
+
+
+def _check_grad(layer, w, gy, gate=None):
+    gx = layer.input_grad(gy, gate=gate)
+    assert gx.dtype == gy.dtype and tuple(gx.shape) == (gy.shape[0], w.shape[1])
+    gd = gy.double().cpu().numpy()
+    ref = R.input_grad(gd, w, None if gate is None else gate.double().cpu().numpy())
+    _check(gx, ref, _tol(ref, np.abs(gd) @ np.abs(w), w.shape[0] + 64, gy.dtype, 2.0 ** -23 if gy.dtype == F32 else 2.0 ** -15))
+
+
+SHAPES = [  # N, K, M, group
+    (1, 1, 1, 32), (1, 32, 16, 32), (2, 31, 17, 32), (1, 2048, 1024, 64), (7, 129, 43, 64), (15, 257, 15, 128),
+    (16, 128, 128, 128), (17, 96, 130, 96), (33, 1000, 129, 160), (100, 2048, 1024, 64), (129, 321, 300, 32),
+    (130, 640, 257, 128), (300, 1024, 43, 64), (1, 5001, 33, 32), (3, 100, 1000, 1024), (257, 511, 385, 256), (600, 64, 10, 32),
+]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shape", SHAPES, ids=["x".join(map(str, s)) for s in SHAPES])
+def test_forward_and_gradient_match_float64(shape, dtype):
+    n, k, m, group = shape
+    i = SHAPES.index(shape)
+    sdt = (F32, dtype, F16)[i % 3]
+    layer, w, b = _layer(m, k, group, sdt, zeros=i % 2 == 0, bias=i % 3 != 1, seed=i)
+    g = torch.Generator().manual_seed(100 + i)
+    _check_forward(layer, w, b, torch.randn((n, k), generator=g).to("cuda", dtype), relu=i % 4 == 3)
+    gate = torch.randn((n, k), generator=g).to("cuda", dtype) if i % 2 else None
+    _check_grad(layer, w, torch.randn((n, m), generator=g).to("cuda", dtype), gate)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n", [1, 5, 40, 300])
+def test_strided_rows_and_untouched_surroundings(n, dtype):
+    k, m = 200, 75
+    layer, w, b = _layer(m, k, 64, bias=True, seed=3)
+    for off, ld in ((0, 256), (1, 203), (3, 201)):          # aligned rows, odd rows, rows that start off a 16-byte border
+        buf = torch.full((n + 1, ld), float("nan"), device="cuda", dtype=dtype)
+        x = buf.as_strided((n, k), (ld, 1), off)
+        x.copy_(torch.randn((n, k), generator=torch.Generator().manual_seed(n)))
+        obuf = torch.full((n + 2, m + 6), 7.0, device="cuda", dtype=dtype)
+        out = obuf[1:n + 1, 2:2 + m]
+        assert layer.forward(x, out=out) is out
+        xd = x.double().cpu().numpy()
+        ref = R.linear(xd, w, b)
+        _check(out, ref, _tol(ref, np.abs(xd) @ np.abs(w).T + np.abs(b), k + 64, dtype))
+        keep = obuf.clone()
+        keep[1:n + 1, 2:2 + m] = 7.0
+        assert bool((keep == 7.0).all())
+        gbuf = torch.full((n + 1, m + 9), float("inf"), device="cuda", dtype=dtype)
+        gy = gbuf.as_strided((n, m), (m + 9, 1), off)
+        gy.copy_(torch.randn((n, m), generator=torch.Generator().manual_seed(n + 1)))
+        xbuf = torch.full((n + 2, k + 5), 7.0, device="cuda", dtype=dtype)
+        gx = xbuf[1:n + 1, 3:3 + k]
+        layer.input_grad(gy, out=gx)
+        gd = gy.double().cpu().numpy()
+        ref = R.input_grad(gd, w)
+        _check(gx, ref, _tol(ref, np.abs(gd) @ np.abs(w), m + 64, dtype, 2.0 ** -15))
+        xbuf[1:n + 1, 3:3 + k] = 7.0
+        assert bool((xbuf == 7.0).all())
+
+
+def test_views_that_are_not_rows_are_copied():
+    layer, w, b = _layer(40, 96, 32, seed=5)
+    x = torch.randn(96, 20, device="cuda")
+    _check_forward(layer, w, b, x.t(), False)
+    _check_forward(layer, w, b, torch.randn(1, 96, device="cuda").expand(9, 96), False)
+    y = layer.forward(torch.randn(2, 3, 96, device="cuda"))
+    assert tuple(y.shape) == (2, 3, 40)
+    assert tuple(layer.forward(torch.empty(0, 96, device="cuda")).shape) == (0, 40)
+    assert tuple(layer.input_grad(torch.empty(0, 40, device="cuda")).shape) == (0, 96)
+    assert tuple(layer.forward(torch.randn(96, device="cuda")).shape) == (40,)
+
+
+@pytest.mark.parametrize("n", [3, 40, 300])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+def test_infinities_stay_in_their_rows(dtype, n):
+    """x[i,k] = inf gives +-inf by the sign of the weight and NaN for a weight of 0, as the formula says; other rows keep
+    their values bit for bit.  A gradient row with an infinity is nowhere finite."""
+    layer, w, b = _layer(70, 130, 32, seed=8)
+    x = torch.randn((n, 130), generator=torch.Generator().manual_seed(1)).to("cuda", dtype)
+    base = layer.forward(x)
+    x2 = x.clone()
+    x2[1, 129] = float("inf")
+    x2[2, 64] = float("nan")
+    y = layer.forward(x2)
+    want = torch.from_numpy(np.where(w[:, 129] > 0, np.inf, np.where(w[:, 129] < 0, -np.inf, np.nan)))
+    assert torch.equal(torch.nan_to_num(y[1].double().cpu(), nan=1.0), torch.nan_to_num(want, nan=1.0))
+    assert bool(torch.isnan(y[2]).all())
+    keep = [i for i in range(n) if i not in (1, 2)]
+    assert torch.equal(y[keep], base[keep])
+    gy = torch.randn((n, 70), generator=torch.Generator().manual_seed(2)).to("cuda", dtype)
+    gbase = layer.input_grad(gy)
+    gy2 = gy.clone()
+    gy2[1, 69] = float("-inf")
+    gy2[2, 3] = float("nan")
+    gx = layer.input_grad(gy2)
+    assert not bool(torch.isfinite(gx[1]).any()) and bool(torch.isnan(gx[2]).all())
+    assert torch.equal(gx[keep], gbase[keep])
+
+
+@pytest.mark.parametrize("n", [2, 300])
+def test_float32_extremes(n):
+    """Activations near both ends of float32's range: the three-piece cut neither overflows nor loses its low pieces."""
+    layer, w, b = _layer(33, 64, 32, zeros=False, seed=9)
+    for scale in (2.0 ** 120, 2.0 ** -90):
+        x = (torch.rand((n, 64), generator=torch.Generator().manual_seed(4)) + 0.5).cuda() * scale
+        _check_forward(layer, w, b, x, False)
+
+
+@pytest.mark.parametrize("n", [1, 20, 300])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_gradient_is_the_forward_difference(n, dtype):
+    """The layer is linear: <gy, f(x + d) - f(x - d)> / 2 = <gx, d> up to the roundings of both sides (64-bit inner
+    products; float32 forward)."""
+    layer, w, b = _layer(150, 260, 64, bias=True, seed=11)
+    g = torch.Generator().manual_seed(7)
+    x, d = torch.randn((n, 260), generator=g).cuda(), torch.randn((n, 260), generator=g).cuda()
+    gy = torch.randn((n, 150), generator=g).cuda().to(dtype)
+    diff = (layer.forward(x + d).double() - layer.forward(x - d).double()) / 2
+    left, right = float((gy.double() * diff).sum()), float((layer.input_grad(gy).double() * d.double()).sum())
+    mag = (gy.double().abs().cpu().numpy() * ((np.abs((x + d).cpu().numpy()) + np.abs((x - d).cpu().numpy())) / 2 @ np.abs(w).T
+                                             + np.abs(b))).sum()
+    gmag = ((gy.double().abs().cpu().numpy() @ np.abs(w)) * np.abs(d.cpu().numpy())).sum()
+    assert abs(left - right) <= mag * 330 * 2.0 ** -23 + gmag * (220 * 2.0 ** -23 + torch.finfo(dtype).eps / 2 + 2.0 ** -15)
+
+
+def test_runs_agree_bit_for_bit_and_streams_do_not_mix():
+    layer, w, b = _layer(300, 700, 64, bias=True, seed=12)
+    xs = [torch.randn((n, 700), device="cuda") for n in (1, 64, 400)]
+    want = [layer.forward(x) for x in xs]
+    gw = [layer.input_grad(y) for y in want]
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    got = []
+    for s in (s1, s2):
+        with torch.cuda.stream(s):
+            got.append([(layer.forward(x), layer.input_grad(y)) for x, y in zip(xs, want)])
+    torch.cuda.synchronize()
+    for ys in got:
+        for (y, g), yw, gww in zip(ys, want, gw):
+            assert torch.equal(y, yw) and torch.equal(g, gww)
+
+
+@pytest.mark.parametrize("n", [1, 40, 300])
+def test_captured_graph_replays(n):
+    layer, w, b = _layer(200, 330, 64, bias=True, seed=13)
+    x = torch.zeros((n, 330), device="cuda", dtype=BF16)
+    y, gx = torch.empty((n, 200), device="cuda", dtype=BF16), torch.empty((n, 330), device="cuda", dtype=BF16)
+    layer.forward(x, out=y)
+    layer.input_grad(y, out=gx)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        layer.forward(x, relu=True, out=y)
+        layer.input_grad(y, gate=x, out=gx)
+    for i in range(4):
+        x.copy_(torch.randn((n, 330), generator=torch.Generator().manual_seed(i)))
+        graph.replay()
+        torch.cuda.synchronize()
+        yw = layer.forward(x, relu=True)
+        assert torch.equal(y, yw) and torch.equal(gx, layer.input_grad(yw, gate=x))
+        torch.cuda.synchronize()
+
+
+def test_quantize_bounds_and_dequantize():
+    g = torch.Generator().manual_seed(0)
+    w = torch.randn((50, 131), generator=g) * torch.rand((50, 1), generator=g)
+    w[3] = 0
+    w[4, :64] = w[4, :64].abs() + 1                                          # a group away from zero
+    for sym in (False, True):
+        q, s, z = quantize(w, 64, sym)
+        back = R.weights(q.numpy(), s.numpy(), None if z is None else z.numpy(), 64, 131)
+        step = s.double().numpy()[:, np.arange(131) // 64]
+        # rounding: half a step; asymmetric: the zero point is rounded too
+        assert (np.abs(back - w.double().numpy()) <= step * (0.5 if sym else 1.0) * 1.0001).all()
+        dq = dequantize(q.cuda(), s.cuda(), None if z is None else z.cuda(), 64, 131)
+        assert np.abs(dq.cpu().double().numpy() - back).max() <= 2.0 ** -24 * np.abs(back).max()
+        layer = LinearW4(q, s, z, group=64, in_features=131)
+        _check_forward(layer, back, None, torch.randn((5, 131), device="cuda"), False)
+
+
+def test_refusals():
+    layer, _, _ = _layer(16, 64, 32)
+    E = _hip.GraphiteHipError
+    q, s = torch.zeros((16, 32), dtype=torch.uint8, device="cuda"), torch.ones((16, 2), device="cuda")
+    for bad in (lambda: LinearW4(q, s, group=48), lambda: LinearW4(q, s, group=0), lambda: LinearW4(q, s, group=64),
+                lambda: LinearW4(q.int(), s, group=32), lambda: LinearW4(q, s.double(), group=32),
+                lambda: LinearW4(q, s, s, group=32), lambda: LinearW4(q, s, group=32, in_features=61),
+                lambda: LinearW4(q, s, group=32, bias=torch.zeros(15)), lambda: LinearW4(q, s, group=32, device="cpu"),
+                lambda: layer.forward(torch.zeros(2, 63, device="cuda")), lambda: layer.forward(torch.zeros(2, 64)),
+                lambda: layer.forward(torch.zeros(2, 64, device="cuda", dtype=torch.float64)),
+                lambda: layer.input_grad(torch.zeros(2, 64, device="cuda")),
+                lambda: layer.input_grad(torch.zeros(2, 16, device="cuda"), gate=torch.zeros(3, 64, device="cuda")),
+                lambda: layer.input_grad(torch.zeros(2, 16, device="cuda"), gate=torch.zeros(2, 64, device="cuda", dtype=F16)),
+                lambda: layer.forward(torch.zeros(2, 64, device="cuda"), out=torch.zeros(2, 15, device="cuda")),
+                lambda: layer.forward(torch.zeros(2, 64, device="cuda"), out=torch.zeros(16, 2, device="cuda").t()),
+                lambda: LinearW4(q, s, group=32, input_grad=False).input_grad(torch.zeros(2, 16, device="cuda"))):
+        with pytest.raises(E):
+            bad()
+
+
+def test_c_entry_refusals():
+    layer, _, _ = _layer(16, 64, 32)
+    lib, ctx = _hip.load_library(), _hip.ctx()
+    x, y = torch.zeros((2, 64), device="cuda"), torch.zeros((2, 16), device="cuda")
+    p, st = _hip._p, _hip._stream()
+    f = lambda **k: lib.gr_linear_w4(ctx, k.get("w", layer._h), k.get("x", p(x)), k.get("dt", 0), k.get("n", 2), k.get("ldx", 64), 0,
+                                     k.get("y", p(y)), k.get("ldy", 16), st)
+    assert f() == 0
+    assert f(n=0, x=None, y=None) == 0
+    for bad in (dict(w=None), dict(x=None), dict(y=None), dict(dt=3), dict(n=-1), dict(ldx=63), dict(ldy=15), dict(n=2 ** 40)):
+        assert f(**bad) == -1 and lib.gr_last_error(ctx)
+    torch.cuda.synchronize()
