@@ -162,8 +162,24 @@ def profile_read():
             for i in range(n)}
 
 
-def _stream(device=None):
-    return _vp(torch.cuda.current_stream(device).cuda_stream)
+def _stream():
+    return _vp(torch.cuda.current_stream().cuda_stream)
+
+
+def op_call(name, device, *args, out=None):
+    """library.name(context of `device`, *args, current stream of `device` [, &out]), with `device` current for the call and the
+    caller's current device left as it was.  The small operators' host path: a few microseconds in all."""
+    dev = device.index
+    c = _ctxs.get(dev) or ctx(dev)
+    fn = getattr(_lib, name)
+    tail = (torch._C._cuda_getCurrentRawStream(dev),) if out is None else (torch._C._cuda_getCurrentRawStream(dev), C.byref(out))
+    if torch.cuda.current_device() == dev:
+        rc = fn(c, *args, *tail)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(c, *args, *tail)
+    if rc != 0:
+        _check(c, rc, name)
 
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # GR_DT_F32, GR_DT_BF16, GR_DT_F16
@@ -178,11 +194,14 @@ def float_rows(t, name, device=None, cols=None):
         raise GraphiteHipError(f"{name} is on {t.device}, expected {device}")
     if t.dtype not in DTYPES:
         raise GraphiteHipError(f"{name} has type {t.dtype}; float32, bfloat16 and float16 are supported")
-    if t.dim() != 2 or (cols is not None and t.shape[1] != cols):
-        raise GraphiteHipError(f"{name} has shape {tuple(t.shape)}, expected [rows, {'columns' if cols is None else cols}]")
-    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+    shape = t.shape
+    if len(shape) != 2 or (cols is not None and shape[1] != cols):
+        raise GraphiteHipError(f"{name} has shape {tuple(shape)}, expected [rows, {'columns' if cols is None else cols}]")
+    st = t.stride()
+    if shape[1] > 1 and st[1] != 1 or shape[0] > 1 and st[0] < shape[1]:
         t = t.contiguous()                      # transposed, reversed or broadcast views
-    return t, (t.stride(0) if t.shape[0] > 1 else max(1, t.shape[1]))
+        st = t.stride()
+    return t, (st[0] if shape[0] > 1 else max(1, shape[1]))
 
 
 def to_dev(a):

@@ -40,13 +40,13 @@ def topk_distill(logits, index, value, tau=1.0, teacher_lse=None, grad_loss=None
         raise _hip.GraphiteHipError(f"index has type {index.dtype}, expected int64")
     if index.device != dev or index.dim() != 2 or index.shape != value.shape or index.shape[1] < 1:
         raise _hip.GraphiteHipError(f"index {tuple(index.shape)} and value {tuple(value.shape)} must be [N, k] tensors on {dev}")
-    shared = index.shape[0] == 1
-    if index.shape[0] != n and not shared:
-        raise _hip.GraphiteHipError(f"index has {index.shape[0]} rows, expected {n} or 1")
-    index = index.contiguous()
-    value, _ = _hip.float_rows(value, "value", dev)
-    value = value.contiguous()
-    rows = 1 if shared else n
+    rows, k = index.shape
+    shared = rows == 1
+    if rows != n and not shared:
+        raise _hip.GraphiteHipError(f"index has {rows} rows, expected {n} or 1")
+    if value.device != dev or value.dtype not in _hip.DTYPES:
+        raise _hip.GraphiteHipError(f"value must be a float32, bfloat16 or float16 tensor on {dev}")
+    index, value = index.contiguous(), value.contiguous()
     for name, t, size in (("teacher_lse", teacher_lse, rows), ("grad_loss", grad_loss, n)):
         if t is not None and (t.device != dev or t.dtype != torch.float32 or t.numel() != size):
             raise _hip.GraphiteHipError(f"{name} must be a float32 tensor of {size} elements on {dev}")
@@ -59,12 +59,8 @@ def topk_distill(logits, index, value, tau=1.0, teacher_lse=None, grad_loss=None
         if grad is not grad_out or grad.dtype != z.dtype or grad.shape[0] != n:
             raise _hip.GraphiteHipError(f"grad_out must be a {z.dtype} tensor [{n}, {v}] with the elements of a row next to each other")
     elif want_grad:
-        grad = torch.empty((n, v), device=dev, dtype=z.dtype)
-    with torch.cuda.device(dev):
-        c = _hip.ctx(dev.index)
-        rc = _hip.load_library().gr_distill_topk(
-            c, _hip._p(z), _hip.DTYPES[z.dtype], n, v, ldz, _hip._p(index), _hip._p(value), _hip.DTYPES[value.dtype],
-            index.shape[1], 0 if shared else index.shape[1], _hip._p(teacher_lse), float(tau), _hip._p(grad_loss), _hip._p(loss),
-            _hip._p(grad), ldg, _hip._stream(dev))
-    _hip._check(c, rc, "gr_distill_topk")
+        grad = z.new_empty((n, v))
+    _hip.op_call("gr_distill_topk", dev, z.data_ptr(), _hip.DTYPES[z.dtype], n, v, ldz, index.data_ptr(), value.data_ptr(),
+                 _hip.DTYPES[value.dtype], k, 0 if shared else k, None if teacher_lse is None else teacher_lse.data_ptr(), float(tau),
+                 None if grad_loss is None else grad_loss.data_ptr(), loss.data_ptr(), None if grad is None else grad.data_ptr(), ldg)
     return loss, grad

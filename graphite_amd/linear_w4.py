@@ -96,64 +96,62 @@ class LinearW4:
         q, scales = q.to(self.device).contiguous(), scales.to(self.device).contiguous()
         zeros = None if zeros is None else zeros.to(self.device).contiguous()
         bias = None if bias is None else bias.to(self.device, torch.float32).contiguous()
-        self._ctx = _hip.ctx(self.device.index)
-        with torch.cuda.device(self.device):
-            rc = _hip.load_library().gr_w4_create(
-                self._ctx, _hip._p(q), q.shape[1], _hip._p(scales), _hip.DTYPES[scales.dtype], want[1], _hip._p(zeros), want[1],
-                _hip._p(bias), self.out_features, k, self.group, int(bool(input_grad)), _hip._stream(self.device), C.byref(self._h))
-        _hip._check(self._ctx, rc, "gr_w4_create")
+        _hip.op_call("gr_w4_create", self.device, q.data_ptr(), q.shape[1], scales.data_ptr(), _hip.DTYPES[scales.dtype], want[1],
+                     zeros.data_ptr() if zeros is not None else None, want[1], bias.data_ptr() if bias is not None else None,
+                     self.out_features, k, self.group, int(bool(input_grad)), out=self._h)
 
     def __del__(self):
         h, self._h = getattr(self, "_h", None), None
         if h and _hip._lib is not None:
             _hip._lib.gr_w4_destroy(h)
 
-    def _out(self, out, n, cols, like, name):
-        if out is None:
-            return torch.empty((n, cols), device=self.device, dtype=like.dtype)
+    def _rows_of(self, out, n, cols, like):
+        """Row stride of a caller's result tensor, after its checks."""
         if out.device != self.device or out.dtype != like.dtype or tuple(out.shape) != (n, cols):
-            raise _hip.GraphiteHipError(f"{name} must be a {like.dtype} tensor [{n}, {cols}] on {self.device}")
+            raise _hip.GraphiteHipError(f"out must be a {like.dtype} tensor [{n}, {cols}] on {self.device}")
         if (cols > 1 and out.stride(1) != 1) or (n > 1 and out.stride(0) < cols):
-            raise _hip.GraphiteHipError(f"{name}: the elements of a row must be next to each other")
-        return out
+            raise _hip.GraphiteHipError("out: the elements of a row must be next to each other")
+        return out.stride(0) if n > 1 else cols
 
     def forward(self, x, relu=False, out=None):
         """x [..., in] -> [..., out] of x's type on the current stream; relu clamps negative results to 0.  Rows of x may be
-        any distance apart.  out: optional result tensor [N, out] (then x is [N, in])."""
-        lead = x.shape[:-1]
+        any distance apart.  out: optional result tensor [rows, out], which must not overlap x."""
+        lead = None
         if x.dim() != 2:
+            lead = x.shape[:-1]
             x = x.reshape(-1, x.shape[-1])
         x, ldx = _hip.float_rows(x, "x", self.device, self.in_features)
-        n = x.shape[0]
-        y = self._out(out, n, self.out_features, x, "out")
-        with torch.cuda.device(self.device):
-            rc = _hip.load_library().gr_linear_w4(self._ctx, self._h, _hip._p(x), _hip.DTYPES[x.dtype], n, ldx, int(bool(relu)),
-                                                  _hip._p(y), y.stride(0) if n > 1 else self.out_features,
-                                                  _hip._stream(self.device))
-        _hip._check(self._ctx, rc, "gr_linear_w4")
-        return y if out is not None else y.view(*lead, self.out_features)
+        n, m = x.shape[0], self.out_features
+        if out is None:
+            y, ldy = x.new_empty((n, m)), m
+        else:
+            y, ldy = out, self._rows_of(out, n, m, x)
+        _hip.op_call("gr_linear_w4", self.device, self._h, x.data_ptr(), _hip.DTYPES[x.dtype], n, ldx, 1 if relu else 0, y.data_ptr(), ldy)
+        return y if out is not None or lead is None else y.view(*lead, m)
 
     __call__ = forward
 
     def input_grad(self, grad_y, gate=None, out=None):
         """grad_y [..., out] -> d loss / d x [..., in] of its type; 0 where gate <= 0 (gate: the rectified activation the
         layer read, shape of the result).  A ReLU of this layer is the caller's to apply to grad_y."""
-        lead = grad_y.shape[:-1]
+        lead = None
         if grad_y.dim() != 2:
+            lead = grad_y.shape[:-1]
             grad_y = grad_y.reshape(-1, grad_y.shape[-1])
         g, ldg = _hip.float_rows(grad_y, "grad_y", self.device, self.out_features)
-        n = g.shape[0]
-        ldgate = self.in_features
+        n, k = g.shape[0], self.in_features
+        gp, ldgate = None, k
         if gate is not None:
             if gate.dtype != g.dtype:
                 raise _hip.GraphiteHipError(f"gate has type {gate.dtype}, expected {g.dtype}")
-            gate, ldgate = _hip.float_rows(gate.reshape(-1, gate.shape[-1]), "gate", self.device, self.in_features)
+            gate, ldgate = _hip.float_rows(gate.reshape(-1, gate.shape[-1]), "gate", self.device, k)
             if gate.shape[0] != n:
                 raise _hip.GraphiteHipError(f"gate has {gate.shape[0]} rows, expected {n}")
-        gx = self._out(out, n, self.in_features, g, "out")
-        with torch.cuda.device(self.device):
-            rc = _hip.load_library().gr_linear_w4_input_grad(
-                self._ctx, self._h, _hip._p(g), _hip.DTYPES[g.dtype], n, ldg, _hip._p(gate), ldgate, _hip._p(gx),
-                gx.stride(0) if n > 1 else self.in_features, _hip._stream(self.device))
-        _hip._check(self._ctx, rc, "gr_linear_w4_input_grad")
-        return gx if out is not None else gx.view(*lead, self.in_features)
+            gp = gate.data_ptr()
+        if out is None:
+            gx, ldgx = g.new_empty((n, k)), k
+        else:
+            gx, ldgx = out, self._rows_of(out, n, k, g)
+        _hip.op_call("gr_linear_w4_input_grad", self.device, self._h, g.data_ptr(), _hip.DTYPES[g.dtype], n, ldg, gp, ldgate,
+                     gx.data_ptr(), ldgx)
+        return gx if out is not None or lead is None else gx.view(*lead, k)
