@@ -266,3 +266,273 @@ __global__ __launch_bounds__(1024) void k_w4_rows(W4Params p) {
         ((T*)p.y)[n * p.ldy + m] = (T)v;
     }
 }
+
+// ---------------------------------------------------------------------------------------------
+// Many rows: LDS-tiled.  A workgroup of WM x WN waves computes (WM*TM*16) output columns x (WN*TN*16) batch rows; a stage of
+// KS * 32 contraction steps is turned into matrix-instruction operands ONCE per workgroup (4-bit weights to integers, f32
+// activations to pieces) on its way global -> registers -> LDS.  LDS holds operands in fragment order ([tile][step][64 lanes]
+// [16 bytes], the order the packed weights already have), so every LDS access is 64 lanes x 16 consecutive bytes.
+// Two LDS buffers, one barrier per stage, global loads one stage ahead.
+// ---------------------------------------------------------------------------------------------
+template <int DT, bool GRAD> struct W4Pieces {          // pieces of the weights and of the activations
+    static constexpr int W = !GRAD ? 1 : DT == GR_DT_F32 ? 3 : 2;
+    static constexpr int X = DT == GR_DT_F32 ? 3 : GRAD && DT == GR_DT_F16 ? 2 : 1;
+    static constexpr int TOP = W > X ? W : X;           // products i, j with i + j < TOP count
+};
+template <int DT, bool GRAD, int TM, int TN, int WM, int WN, int KS>
+struct W4Gemm {
+    using P = W4Pieces<DT, GRAD>;
+    static constexpr int NT = WM * WN * 64, BM = WM * TM * 16, BN = WN * TN * 16;
+    static constexpr int A_ONE = BM / 16 * KS * 64, X_ONE = BN / 16 * KS * 64;      // 16-byte slots of one piece
+    static constexpr int SLOTS = A_ONE * P::W + X_ONE * P::X;
+    static constexpr int LDS = 2 * SLOTS * 16;
+    static constexpr int AV = BM / 16 * 64 / NT, XV = X_ONE / NT;
+    static_assert(BM / 16 * 64 % NT == 0 && X_ONE % NT == 0, "stage loads must divide evenly");
+    static_assert(LDS <= 160 * 1024, "LDS");
+};
+
+template <int DT, bool GRAD, int TM, int TN, int WM, int WN, int KS>
+__global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
+    using G = W4Gemm<DT, GRAD, TM, TN, WM, WN, KS>;
+    using P = typename G::P;
+    typedef typename W4Type<DT>::T T;
+    constexpr bool F16OP = !GRAD && DT == GR_DT_F16;     // f16 matrix instructions; bf16 otherwise
+    extern __shared__ __attribute__((aligned(16))) w4_u32x4 w4_lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int wm = wave % WM, wn = wave / WM, lr = lane & 15, lh = lane >> 4;
+    // workgroups go round the 8 dies; each die takes a contiguous run of tiles, so that its L2 serves neighbouring ones
+    const int nmt = (p.R + G::BM - 1) / G::BM;
+    const unsigned nb = gridDim.x, per = nb / 8, die = blockIdx.x % 8, seq = blockIdx.x / 8;
+    const unsigned tile = seq < per ? die * per + seq : blockIdx.x;          // the last nb % 8 keep their number
+    const int m0 = (int)(tile % nmt) * G::BM;
+    const int64_t n0 = (int64_t)(tile / nmt) * G::BN;
+    const int nstages = (p.C + KS * 32 - 1) / (KS * 32);
+
+    // ---- staging: thread's share of the weights (AV packed lanes) and of the activations (XV runs of eight)
+    unsigned wreg[G::AV][KS];
+    T xreg[G::XV][8];
+    float zreg[GRAD ? 1 : G::AV][KS];
+    const T* xrow[G::XV];
+    int xk[G::XV];
+    bool xlive[G::XV];
+#pragma unroll
+    for (int v = 0; v < G::XV; v++) {
+        const int f = tid + v * G::NT, l = f & 63, ts = f >> 6;
+        const int64_t n = n0 + ts / KS * 16 + (l & 15);
+        xlive[v] = n < p.N;
+        xrow[v] = (const T*)p.x + (xlive[v] ? n : 0) * p.ldx;
+        xk[v] = ts % KS * 32 + (l >> 4) * 8;
+    }
+    size_t grow[G::AV];                                   // GRAD: scales / zeros of the thread's row
+#pragma unroll
+    for (int v = 0; v < G::AV; v++) {
+        const int row = m0 + (tid + v * G::NT) / 64 * 16 + lr;
+        grow[v] = (size_t)((row < p.R ? row : p.R - 1) / (p.gsteps * 32)) * p.Mp;
+    }
+    int zg = 0, zrem = 0;                                 // group of the next step to load
+    auto load = [&](int s) {
+#pragma unroll
+        for (int v = 0; v < G::AV; v++) {
+            const size_t rt = m0 / 16 + (tid + v * G::NT) / 64;
+            const unsigned* src = (const unsigned*)(p.pack + (rt * p.chunks + s * KS / 4) * 64 + lane) + s * KS % 4;
+            if constexpr (KS == 2) {
+                const uint2 d = *(const uint2*)src;
+                wreg[v][0] = d.x; wreg[v][1] = d.y;
+            } else {
+                wreg[v][0] = *src;
+            }
+        }
+        if constexpr (!GRAD) {
+#pragma unroll
+            for (int i = 0; i < KS; i++) {
+#pragma unroll
+                for (int v = 0; v < G::AV; v++)
+                    zreg[v][i] = p.zeros ? (float)p.zeros[(size_t)zg * p.Mp + m0 + (tid + v * G::NT) / 64 * 16 + lr] : 8.f;
+                if (++zrem == p.gsteps) { zrem = 0; if ((s * KS + i + 1) * 32 < p.C) zg++; }
+            }
+        }
+#pragma unroll
+        for (int v = 0; v < G::XV; v++) w4_load8<DT>(xrow[v], s * KS * 32 + xk[v], p.C, xlive[v], p.xvec != 0, xreg[v]);
+    };
+    auto store = [&](int s, w4_u32x4* buf) {
+#pragma unroll
+        for (int v = 0; v < G::AV; v++) {
+            const int rt = (tid + v * G::NT) / 64;
+#pragma unroll
+            for (int i = 0; i < KS; i++) {
+                w4_u32x4* dst = buf + (rt * KS + i) * 64 + lane;
+                if constexpr (F16OP) {
+                    union { w4_f16x8 h; w4_u32x4 u; } c;
+                    c.h = w4_ints_f16(wreg[v][i], zreg[v][i]);
+                    dst[0] = c.u;
+                } else if constexpr (!GRAD) {
+                    union { w4_bf16x8 h; w4_u32x4 u; } c;
+                    c.h = w4_ints_bf16(wreg[v][i], zreg[v][i]);
+                    dst[0] = c.u;
+                } else {
+                    const size_t mb = grow[v] + s * KS * 32 + i * 32 + lh * 8;
+                    float f[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const int q = (int)(wreg[v][i] >> (4 * ((e >> 1) + 4 * (e & 1)))) & 15;
+                        f[e] = ((float)q - (p.zeros ? (float)p.zeros[mb + e] : 8.f)) * w4_scale(p.scales, p.st, mb + e);
+                    }
+                    w4_bf16x8 pc[P::W];
+                    w4_pieces<P::W>(f, pc);
+#pragma unroll
+                    for (int q = 0; q < P::W; q++) {
+                        union { w4_bf16x8 h; w4_u32x4 u; } c;
+                        c.h = pc[q];
+                        dst[q * G::A_ONE] = c.u;
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int v = 0; v < G::XV; v++) {
+            w4_u32x4* dst = buf + P::W * G::A_ONE + tid + v * G::NT;
+            if constexpr (P::X == 1) {
+                union { T t[8]; w4_u32x4 u; } c;
+#pragma unroll
+                for (int e = 0; e < 8; e++) c.t[e] = xreg[v][e];
+                dst[0] = c.u;
+            } else {
+                float f[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) f[e] = (float)xreg[v][e];
+                w4_bf16x8 pc[P::X];
+                w4_pieces<P::X>(f, pc);
+#pragma unroll
+                for (int q = 0; q < P::X; q++) {
+                    union { w4_bf16x8 h; w4_u32x4 u; } c;
+                    c.h = pc[q];
+                    dst[q * G::X_ONE] = c.u;
+                }
+            }
+        }
+    };
+
+    w4_f32x4 acc[TM][TN], part[GRAD ? 1 : TM][GRAD ? 1 : TN];
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+        for (int j = 0; j < TN; j++) acc[i][j] = w4_f32x4{0.f, 0.f, 0.f, 0.f};
+    const w4_f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
+    union Frag { w4_u32x4 u; w4_bf16x8 b; w4_f16x8 h; };
+    int cg = 0, crem = 0;                                 // group of the step being multiplied
+    auto step = [&](const w4_u32x4* buf, int i, bool last) {
+        Frag a[P::W][TM], x[P::X][TN];
+#pragma unroll
+        for (int q = 0; q < P::W; q++)
+#pragma unroll
+            for (int t = 0; t < TM; t++) a[q][t].u = buf[q * G::A_ONE + ((wm * TM + t) * KS + i) * 64 + lane];
+#pragma unroll
+        for (int q = 0; q < P::X; q++)
+#pragma unroll
+            for (int t = 0; t < TN; t++) x[q][t].u = buf[P::W * G::A_ONE + q * G::X_ONE + ((wn * TN + t) * KS + i) * 64 + lane];
+        auto mul = [&](int qa, int qx, int t, int u, w4_f32x4 c) {
+            if constexpr (F16OP) return w4_mfma(a[qa][t].h, x[qx][u].h, c);
+            else return w4_mfma(a[qa][t].b, x[qx][u].b, c);
+        };
+        if constexpr (GRAD) {
+#pragma unroll
+            for (int qa = 0; qa < P::W; qa++)
+#pragma unroll
+                for (int qx = 0; qx < P::X; qx++) {
+                    if (qa + qx >= P::TOP) continue;
+#pragma unroll
+                    for (int t = 0; t < TM; t++)
+#pragma unroll
+                        for (int u = 0; u < TN; u++) acc[t][u] = mul(qa, qx, t, u, acc[t][u]);
+                }
+        } else {
+            const bool flush = crem + 1 == p.gsteps || last;
+            float sc[TM][4];
+            if (flush) {
+#pragma unroll
+                for (int t = 0; t < TM; t++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        sc[t][r] = w4_scale(p.scales, p.st, (size_t)cg * p.Mp + m0 + (wm * TM + t) * 16 + lh * 4 + r);
+            }
+            if (crem == 0) {
+#pragma unroll
+                for (int t = 0; t < TM; t++)
+#pragma unroll
+                    for (int u = 0; u < TN; u++) part[t][u] = mul(0, 0, t, u, zero4);
+            } else {
+#pragma unroll
+                for (int t = 0; t < TM; t++)
+#pragma unroll
+                    for (int u = 0; u < TN; u++) part[t][u] = mul(0, 0, t, u, part[t][u]);
+            }
+#pragma unroll
+            for (int qx = 1; qx < P::X; qx++)
+#pragma unroll
+                for (int t = 0; t < TM; t++)
+#pragma unroll
+                    for (int u = 0; u < TN; u++) part[t][u] = mul(0, qx, t, u, part[t][u]);
+            crem++;
+            if (flush) {
+#pragma unroll
+                for (int t = 0; t < TM; t++)
+#pragma unroll
+                    for (int u = 0; u < TN; u++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) acc[t][u][r] = __builtin_fmaf(part[t][u][r], sc[t][r], acc[t][u][r]);
+                crem = 0;
+                cg++;
+            }
+        }
+    };
+
+    load(0);
+    store(0, w4_lds);
+    if (nstages > 1) load(1);
+    __syncthreads();
+    for (int s = 0; s < nstages; s++) {
+        if (s + 1 < nstages) {
+            store(s + 1, w4_lds + ((s + 1) & 1) * G::SLOTS);
+            if (s + 2 < nstages) load(s + 2);
+        }
+        const w4_u32x4* buf = w4_lds + (s & 1) * G::SLOTS;
+#pragma unroll
+        for (int i = 0; i < KS; i++) {
+            if (i > 0 && (s * KS + i) * 32 >= p.C) break;
+            step(buf, i, (s * KS + i + 1) * 32 >= p.C);
+        }
+        __syncthreads();
+    }
+
+    const bool vec = ((uintptr_t)p.y % (4 * sizeof(T)) == 0) && p.ldy % 4 == 0;
+#pragma unroll
+    for (int u = 0; u < TN; u++) {
+        const int64_t n = n0 + (wn * TN + u) * 16 + lr;
+        if (n >= p.N) continue;
+#pragma unroll
+        for (int t = 0; t < TM; t++) {
+            const int m = m0 + (wm * TM + t) * 16 + lh * 4;
+            float v[4];
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                v[r] = acc[t][u][r];
+                if (m + r >= p.R) continue;
+                if constexpr (!GRAD) {
+                    if (p.bias) v[r] += p.bias[m + r];
+                    if (p.relu) v[r] = v[r] < 0.f ? 0.f : v[r];
+                } else if (p.gate) {
+                    v[r] = (float)((const T*)p.gate)[n * p.ldg + m + r] > 0.f ? v[r] : 0.f;
+                }
+            }
+            T* dst = (T*)p.y + n * p.ldy + m;
+            if (vec && m + 4 <= p.R) {
+                struct alignas(4 * sizeof(T)) T4 { T t[4]; } o = {{(T)v[0], (T)v[1], (T)v[2], (T)v[3]}};
+                *(T4*)dst = o;
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    if (m + r < p.R) dst[r] = (T)v[r];
+            }
+        }
+    }
+}

@@ -120,10 +120,24 @@ static void launch_rows(const W4Params& p, hipStream_t st) {
     if (waves > p.chunks) waves = p.chunks;
     hipLaunchKernelGGL((k_w4_rows<DT, NT, MT, GRAD>), dim3((unsigned)blocks), dim3(waves * 64), (size_t)waves * MT * NT * 1024, st, p);
 }
+template <int DT, bool GRAD, int TM, int TN, int WM, int WN, int KS>
+static hipError_t launch_gemm(const W4Params& p, hipStream_t st) {
+    using G = W4Gemm<DT, GRAD, TM, TN, WM, WN, KS>;
+    auto kern = &k_w4_gemm<DT, GRAD, TM, TN, WM, WN, KS>;
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, G::LDS);
+    if (e != hipSuccess) return e;
+    const int64_t blocks = (int64_t)((p.R + G::BM - 1) / G::BM) * ((p.N + G::BN - 1) / G::BN);
+    hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(G::NT), G::LDS, st, p);
+    return hipGetLastError();
+}
 template <int DT, bool GRAD>
-static void launch_any(const W4Params& p, hipStream_t st) {
+static hipError_t launch_any(const W4Params& p, hipStream_t st) {
     if (p.N <= 16) launch_rows<DT, 1, GRAD>(p, st);
-    else launch_rows<DT, 2, GRAD>(p, st);
+    else if (p.N <= 200) launch_rows<DT, 2, GRAD>(p, st);
+    else if constexpr (GRAD && DT == GR_DT_F32) return launch_gemm<DT, GRAD, 4, 2, 2, 4, 1>(p, st);
+    else if constexpr (DT == GR_DT_F32 || (GRAD && DT == GR_DT_F16)) return launch_gemm<DT, GRAD, 4, 2, 2, 4, 2>(p, st);
+    else return launch_gemm<DT, GRAD, 4, 4, 2, 4, 2>(p, st);
+    return hipGetLastError();
 }
 
 static int w4_run(gr_ctx* ctx, const gr_w4* w, const char* who, bool grad, const void* x, int dt, int64_t N, int64_t ldx, const void* gate,
@@ -152,15 +166,16 @@ static int w4_run(gr_ctx* ctx, const gr_w4* w, const char* who, bool grad, const
     const double fl = 2.0 * (double)N * w->M * w->K;
     const double by = (double)w->M * w->K / 2 + (double)w->M * w->G * (dt_size(w->st) + (w->zeros ? 1 : 0)) + (double)N * (w->M + w->K) * es;
     ProfScope ps(ctx, grad ? "k_w4_grad" : "k_w4_forward", st, fl, by);
+    hipError_t e;
     switch (dt * 2 + (grad ? 1 : 0)) {
-        case GR_DT_F32 * 2: launch_any<GR_DT_F32, false>(p, st); break;
-        case GR_DT_F32 * 2 + 1: launch_any<GR_DT_F32, true>(p, st); break;
-        case GR_DT_BF16 * 2: launch_any<GR_DT_BF16, false>(p, st); break;
-        case GR_DT_BF16 * 2 + 1: launch_any<GR_DT_BF16, true>(p, st); break;
-        case GR_DT_F16 * 2: launch_any<GR_DT_F16, false>(p, st); break;
-        default: launch_any<GR_DT_F16, true>(p, st); break;
+        case GR_DT_F32 * 2: e = launch_any<GR_DT_F32, false>(p, st); break;
+        case GR_DT_F32 * 2 + 1: e = launch_any<GR_DT_F32, true>(p, st); break;
+        case GR_DT_BF16 * 2: e = launch_any<GR_DT_BF16, false>(p, st); break;
+        case GR_DT_BF16 * 2 + 1: e = launch_any<GR_DT_BF16, true>(p, st); break;
+        case GR_DT_F16 * 2: e = launch_any<GR_DT_F16, false>(p, st); break;
+        default: e = launch_any<GR_DT_F16, true>(p, st); break;
     }
-    GR_HIP(ctx, hipGetLastError());
+    GR_HIP(ctx, e);
     return GR_OK;
 }
 
