@@ -30,9 +30,8 @@ constexpr int W4_CHUNK = 128;         // contraction steps of a tile
 
 struct W4Params {
     const w4_u32x4* pack;    // [row tiles][chunks][64]
-    const void* scales;      // [groups][Mp], type st
+    const void* scales;      // [groups][Mp], type ST of the kernel
     const uint8_t* zeros;    // [groups][Mp], or null: 8 everywhere
-    int st;
     int Mp;                  // padded out_features
     int chunks;              // of the contraction
     int C, R;                // contraction length, output columns (true sizes)
@@ -43,7 +42,6 @@ struct W4Params {
     const void* gate;        // [N][R], row stride ldg, or null (gradient): output 0 where gate <= 0
     int64_t N, ldx, ldy, ldg;
     int relu;
-    int xvec;                // x rows are 16-byte aligned
 };
 
 template <int DT> struct W4Type;
@@ -51,33 +49,36 @@ template <> struct W4Type<GR_DT_F32> { typedef float T; };
 template <> struct W4Type<GR_DT_BF16> { typedef __bf16 T; };
 template <> struct W4Type<GR_DT_F16> { typedef _Float16 T; };
 
-__device__ __forceinline__ float w4_scale(const void* s, int st, size_t i) {
-    if (st == GR_DT_F32) return ((const float*)s)[i];
-    if (st == GR_DT_BF16) return (float)((const __bf16*)s)[i];
-    return (float)((const _Float16*)s)[i];
-}
-
 __device__ __forceinline__ unsigned w4_pack_hi(float a, float b) {       // high halves of a (low) and b (high)
     return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
 }
-// eight nibbles - z as bf16 (exact: |v| <= 15)
-__device__ __forceinline__ w4_bf16x8 w4_ints_bf16(unsigned w, const float (&z)[8]) {
+// Two nibbles as float, minus z: nibbles p and p + 4 of w become the halves 1024 + q of an f16 pair (q sits in the lowest
+// mantissa bits), and one mixed-precision fma per element converts and subtracts.  Exact.
+__device__ __forceinline__ void w4_ints_f32(unsigned w, int p, float z0, float z1, float& a, float& b) {
+    union { unsigned u; w4_f16x2 h; } c;
+    c.u = ((w >> (4 * p)) & 0x000f000fu) | 0x64006400u;
+    a = __builtin_fmaf((float)c.h[0], 1.f, -z0);
+    b = __builtin_fmaf((float)c.h[1], 1.f, -z1);
+}
+// eight nibbles - z as bf16 (exact: |v| <= 15); zk = 1024 + z
+__device__ __forceinline__ w4_bf16x8 w4_ints_bf16(unsigned w, const float (&zk)[8]) {
     union { unsigned u[4]; w4_bf16x8 v; } o;
 #pragma unroll
     for (int p = 0; p < 4; p++) {
-        const float a = (float)((w >> (4 * p)) & 15u) - z[2 * p], b = (float)((w >> (4 * p + 16)) & 15u) - z[2 * p + 1];
+        float a, b;
+        w4_ints_f32(w, p, zk[2 * p], zk[2 * p + 1], a, b);
         o.u[p] = w4_pack_hi(a, b);
     }
     return o.v;
 }
-__device__ __forceinline__ w4_bf16x8 w4_ints_bf16(unsigned w, float z) {
-    const float zz[8] = {z, z, z, z, z, z, z, z};
+__device__ __forceinline__ w4_bf16x8 w4_ints_bf16(unsigned w, float zk) {
+    const float zz[8] = {zk, zk, zk, zk, zk, zk, zk, zk};
     return w4_ints_bf16(w, zz);
 }
-// the same as f16: 1024 + q has q in its lowest bits, and 1024 + q - (1024 + z) is exact
-__device__ __forceinline__ w4_f16x8 w4_ints_f16(unsigned w, float z) {
+// the same as f16: 1024 + q - (1024 + z), a packed subtraction
+__device__ __forceinline__ w4_f16x8 w4_ints_f16(unsigned w, float zk) {
     union { unsigned u[4]; w4_f16x2 h[4]; w4_f16x8 v; } o;
-    const _Float16 zh = (_Float16)(1024.f + z);
+    const _Float16 zh = (_Float16)zk;
     const w4_f16x2 zz = {zh, zh};
 #pragma unroll
     for (int p = 0; p < 4; p++) {
@@ -86,20 +87,14 @@ __device__ __forceinline__ w4_f16x8 w4_ints_f16(unsigned w, float z) {
     }
     return o.v;
 }
-// v = p0 + p1 (+ p2) with bf16 pieces, each cut from what the ones before leave, the last one rounded: three pieces are
-// exact, two leave at most 2^-15 |v|.  An infinity or NaN stays in p0 alone.
+// v = p0 + p1 (+ p2) with bf16 pieces, each cut from what the ones before leave, the last one of two rounded: three pieces are
+// exact, two leave at most 2^-15 |v|.  An infinity stays in p0 alone.
 template <int P>
 __device__ __forceinline__ void w4_pieces(const float (&v)[8], w4_bf16x8 (&out)[P]) {
     union { unsigned u[4]; w4_bf16x8 b; } o[P];
 #pragma unroll
     for (int h = 0; h < 4; h++) {
         float r[2] = {v[2 * h], v[2 * h + 1]};
-        bool fin[2];
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            fin[i] = __builtin_fabsf(r[i]) < __builtin_inff();
-            if (r[i] != r[i]) r[i] = __uint_as_float(0x7fc00000u);
-        }
 #pragma unroll
         for (int p = 0; p < P; p++) {
             if (p == 1 && P == 2) {
@@ -110,136 +105,242 @@ __device__ __forceinline__ void w4_pieces(const float (&v)[8], w4_bf16x8 (&out)[
             if (p == P - 1) continue;
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const float t = __uint_as_float(__float_as_uint(r[i]) & 0xffff0000u);
-                r[i] = fin[i] ? r[i] - t : 0.f;
+                const float d = r[i] - __uint_as_float(__float_as_uint(r[i]) & 0xffff0000u);
+                r[i] = p == 0 && __builtin_fabsf(r[i]) == __builtin_inff() ? 0.f : d;
             }
         }
     }
 #pragma unroll
     for (int p = 0; p < P; p++) out[p] = o[p].b;
 }
-// eight consecutive values of a row, zero beyond C
-template <int DT>
-__device__ __forceinline__ void w4_load8(const typename W4Type<DT>::T* row, int k, int C, bool live, bool vec,
-                                         typename W4Type<DT>::T (&v)[8]) {
+
+// Eight consecutive elements of a row, as loaded.  Rows need no alignment beyond their elements' (the hardware takes 16-byte
+// loads at any element).
+typedef unsigned w4_u32x4_u __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned w4_u32x2_u __attribute__((ext_vector_type(2), aligned(2)));
+template <int DT> struct W4Raw {
+    static constexpr int Q = DT == GR_DT_F32 ? 2 : 1;
     typedef typename W4Type<DT>::T T;
-    if (live && vec && k + 8 <= C) {
-        union { w4_u32x4 q[sizeof(T) / 2]; T t[8]; } u;
+    w4_u32x4 q[Q];
+    __device__ __forceinline__ void load(const T* src) {
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; i++) u.q[i] = ((const w4_u32x4*)(row + k))[i];
-#pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = u.t[e];
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = (live && k + e < C) ? row[k + e] : (T)0.f;
+        for (int i = 0; i < Q; i++) q[i] = *(const w4_u32x4_u*)(src + i * (16 / (int)sizeof(T)));
     }
-}
+    // zero from `count` on (count <= 0: all); what is read there instead is the row's last element
+    __device__ __forceinline__ void load_part(const T* src, int count) {
+        union { w4_u32x4 q[Q]; T t[8]; } u;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const T v = src[e < count ? e : count - 1];
+            u.t[e] = e < count ? v : (T)0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < Q; i++) q[i] = u.q[i];
+    }
+    __device__ __forceinline__ void get(float (&f)[8]) const {
+        if constexpr (DT == GR_DT_F32) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) f[e] = __uint_as_float(q[e / 4][e % 4]);
+        } else if constexpr (DT == GR_DT_BF16) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) f[e] = __uint_as_float(e % 2 ? q[0][e / 2] & 0xffff0000u : q[0][e / 2] << 16);
+        } else {
+            union { w4_u32x4 u; _Float16 h[8]; } c;
+            c.u = q[0];
+#pragma unroll
+            for (int e = 0; e < 8; e++) f[e] = (float)c.h[e];
+        }
+    }
+    __device__ __forceinline__ w4_bf16x8 bf16() const { union { w4_u32x4 u; w4_bf16x8 b; } c; c.u = q[0]; return c.b; }
+    __device__ __forceinline__ w4_f16x8 f16() const { union { w4_u32x4 u; w4_f16x8 b; } c; c.u = q[0]; return c.b; }
+};
+// four scales of consecutive rows (16- or 8-byte aligned)
+template <int ST> struct W4Scale4 {
+    typedef typename W4Type<ST>::T T;
+    typedef T V __attribute__((ext_vector_type(4)));
+    V v;
+    __device__ __forceinline__ void load(const void* s, size_t i) { v = *(const V*)((const T*)s + i); }
+    __device__ __forceinline__ float operator[](int r) const { return (float)v[r]; }
+};
 __device__ __forceinline__ w4_f32x4 w4_mfma(w4_bf16x8 a, w4_bf16x8 b, w4_f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 __device__ __forceinline__ w4_f32x4 w4_mfma(w4_f16x8 a, w4_f16x8 b, w4_f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
+// the sum v of output m of row n, through the epilogue, to memory
+template <int DT, bool GRAD>
+__device__ __forceinline__ typename W4Type<DT>::T w4_finish(const W4Params& p, float v, int64_t n, int m) {
+    typedef typename W4Type<DT>::T T;
+    if constexpr (!GRAD) {
+        if (p.bias) v += p.bias[m];
+        if (p.relu) v = v < 0.f ? 0.f : v;
+    } else if (p.gate) {
+        v = (float)((const T*)p.gate)[n * p.ldg + m] > 0.f ? v : 0.f;
+    }
+    return (T)v;
+}
 
-// Few rows.  A workgroup owns MT row tiles x NT tiles of 16 batch rows; its waves take the contraction's chunks in turn and
-// their sums meet in LDS, in wave order.
-template <int DT, int NT, int MT, bool GRAD>
-__global__ __launch_bounds__(1024) void k_w4_rows(W4Params p) {
+// ---------------------------------------------------------------------------------------------
+// Few rows.  A workgroup owns MT row tiles x NT tiles of 16 batch rows; its waves take the contraction's chunks in turn, D
+// chunks at a time (all their loads are issued before the first is used), and their sums meet in LDS, in wave order.
+// Forward: GS = groups of a chunk (1, 2 or 4; 4 also where a border falls on any step).
+// ---------------------------------------------------------------------------------------------
+constexpr int w4_rows_waves(int nt, bool grad) { return nt > 1 && grad ? 8 : 16; }      // the most a workgroup may have
+template <int DT, int ST, int NT, int MT, int GS, int D, bool GRAD>
+__global__ __launch_bounds__(w4_rows_waves(NT, GRAD) * 64) void k_w4_rows(W4Params p) {
     typedef typename W4Type<DT>::T T;
     extern __shared__ __attribute__((aligned(16))) float w4_red[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nwaves = blockDim.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nwaves = blockDim.x >> 6;
     const int lr = lane & 15, lh = lane >> 4;
     const int nmt = (p.R + 16 * MT - 1) / (16 * MT);
     const int rt0 = (int)(blockIdx.x % nmt) * MT;
     const int64_t n0 = (int64_t)(blockIdx.x / nmt) * (16 * NT);
     const T* xrow[NT];
-    bool live[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) {
         const int64_t n = n0 + t * 16 + lr;
-        live[t] = n < p.N;
-        xrow[t] = (const T*)p.x + (live[t] ? n : 0) * p.ldx;
+        xrow[t] = (const T*)p.x + (n < p.N ? n : p.N - 1) * p.ldx + lh * 8;      // columns beyond the batch: computed, not stored
     }
+    const size_t grow = GRAD ? (size_t)((rt0 >> 1) / p.gsteps) * p.Mp : 0;        // group of the rows (MT is 1 or 2)
     w4_f32x4 acc[MT][NT];
 #pragma unroll
     for (int a = 0; a < MT; a++)
 #pragma unroll
         for (int t = 0; t < NT; t++) acc[a][t] = w4_f32x4{0.f, 0.f, 0.f, 0.f};
 
-    for (int c = wave; c < p.chunks; c += nwaves) {
+    struct Chunk {
         w4_u32x4 w[MT];
+        W4Raw<DT> x[4][NT];
+        W4Scale4<ST> s[GRAD ? 1 : GS][MT];
+        uint8_t z[GRAD ? 1 : GS][MT];
+        W4Raw<ST> gs[GRAD ? 4 : 1];
+        uint2 gz[GRAD ? 4 : 1];
+    };
+    auto load = [&](Chunk& h, int c) {
+        const int kb = c * W4_CHUNK;
 #pragma unroll
-        for (int a = 0; a < MT; a++) w[a] = p.pack[((size_t)(rt0 + a) * p.chunks + c) * 64 + lane];
+        for (int a = 0; a < MT; a++) h.w[a] = p.pack[((size_t)(rt0 + a) * p.chunks + c) * 64 + lane];
+        if (kb + W4_CHUNK <= p.C) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int kb = c * W4_CHUNK + i * 32;
-            if (kb >= p.C) break;
-            T xv[NT][8];
+            for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int t = 0; t < NT; t++) w4_load8<DT>(xrow[t], kb + lh * 8, p.C, live[t], p.xvec != 0, xv[t]);
-            if constexpr (!GRAD) {
-                const size_t gb = (size_t)((kb >> 5) / p.gsteps) * p.Mp;
+                for (int t = 0; t < NT; t++) h.x[i][t].load(xrow[t] + kb + i * 32);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int t = 0; t < NT; t++) h.x[i][t].load_part(xrow[t] + kb + i * 32, p.C - kb - i * 32 - lh * 8);
+        }
+        if constexpr (!GRAD) {
+#pragma unroll
+            for (int g = 0; g < GS; g++) {
+                int step = c * 4 + g * (4 / GS);
+                if (step * 32 >= p.C) step = c * 4;                               // beyond the row: x is 0 there
+                const size_t row = (size_t)(step / p.gsteps) * p.Mp + (size_t)rt0 * 16;
 #pragma unroll
                 for (int a = 0; a < MT; a++) {
-                    const size_t row = gb + (size_t)(rt0 + a) * 16;
-                    const float z = p.zeros ? (float)p.zeros[row + lr] : 8.f;
-                    float s[4];
+                    h.s[g][a].load(p.scales, row + a * 16 + lh * 4);
+                    h.z[g][a] = p.zeros ? p.zeros[row + a * 16 + lr] : 8;
+                }
+            }
+        } else {
 #pragma unroll
-                    for (int r = 0; r < 4; r++) s[r] = w4_scale(p.scales, p.st, row + lh * 4 + r);
+            for (int i = 0; i < 4; i++) {
+                const size_t mb = grow + kb + i * 32 + lh * 8;
+                h.gs[i].load((const typename W4Type<ST>::T*)p.scales + mb);
+                h.gz[i] = p.zeros ? *(const uint2*)(p.zeros + mb) : uint2{0x08080808u, 0x08080808u};
+            }
+        }
+    };
+    auto mul = [&](const Chunk& h) {
+        if constexpr (!GRAD) {
 #pragma unroll
-                    for (int t = 0; t < NT; t++) {
-                        w4_f32x4 part = {0.f, 0.f, 0.f, 0.f};
-                        if constexpr (DT == GR_DT_F32) {
-                            w4_bf16x8 pc[3];
-                            w4_pieces<3>(xv[t], pc);
-                            const w4_bf16x8 wi = w4_ints_bf16(w[a][i], z);
+            for (int g = 0; g < GS; g++) {
+                w4_f32x4 part[MT][NT];
 #pragma unroll
-                            for (int q = 0; q < 3; q++) part = w4_mfma(wi, pc[q], part);
-                        } else {
-                            if constexpr (DT == GR_DT_BF16) {
-                                union { T t8[8]; w4_bf16x8 v; } u;
+                for (int a = 0; a < MT; a++)
 #pragma unroll
-                                for (int e = 0; e < 8; e++) u.t8[e] = xv[t][e];
-                                part = w4_mfma(w4_ints_bf16(w[a][i], z), u.v, part);
-                            } else {
-                                union { T t8[8]; w4_f16x8 v; } u;
+                    for (int t = 0; t < NT; t++) part[a][t] = w4_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                                for (int e = 0; e < 8; e++) u.t8[e] = xv[t][e];
-                                part = w4_mfma(w4_ints_f16(w[a][i], z), u.v, part);
-                            }
+                for (int i = g * (4 / GS); i < (g + 1) * (4 / GS); i++) {
+                    if constexpr (DT == GR_DT_F16) {
+#pragma unroll
+                        for (int a = 0; a < MT; a++) {
+                            const w4_f16x8 wi = w4_ints_f16(h.w[a][i], 1024.f + (float)h.z[g][a]);
+#pragma unroll
+                            for (int t = 0; t < NT; t++) part[a][t] = w4_mfma(wi, h.x[i][t].f16(), part[a][t]);
                         }
+                    } else {
+                        w4_bf16x8 wi[MT];
 #pragma unroll
-                        for (int r = 0; r < 4; r++) acc[a][t][r] = __builtin_fmaf(part[r], s[r], acc[a][t][r]);
+                        for (int a = 0; a < MT; a++) wi[a] = w4_ints_bf16(h.w[a][i], 1024.f + (float)h.z[g][a]);
+#pragma unroll
+                        for (int t = 0; t < NT; t++) {
+                            constexpr int P = DT == GR_DT_F32 ? 3 : 1;
+                            w4_bf16x8 pc[P];
+                            if constexpr (P == 3) {
+                                float f[8];
+                                h.x[i][t].get(f);
+                                w4_pieces<3>(f, pc);
+                            } else {
+                                pc[0] = h.x[i][t].bf16();
+                            }
+#pragma unroll
+                            for (int q = 0; q < P; q++)
+#pragma unroll
+                                for (int a = 0; a < MT; a++) part[a][t] = w4_mfma(wi[a], pc[q], part[a][t]);
+                        }
                     }
                 }
-            } else {
-                constexpr int P = DT == GR_DT_F32 ? 3 : 2;
-                const size_t mb = (size_t)(rt0 >> 1) / p.gsteps * p.Mp + kb + lh * 8;      // rt0 * 16 / group: MT is 1 or 2
-                float s[8], z[8];
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    s[e] = w4_scale(p.scales, p.st, mb + e);
-                    z[e] = p.zeros ? (float)p.zeros[mb + e] : 8.f;
-                }
-                w4_bf16x8 pc[NT][P];
-#pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    float g[8];
-#pragma unroll
-                    for (int e = 0; e < 8; e++) g[e] = (float)xv[t][e] * s[e];
-                    w4_pieces<P>(g, pc[t]);
-                }
-#pragma unroll
-                for (int a = 0; a < MT; a++) {
-                    const w4_bf16x8 wi = w4_ints_bf16(w[a][i], z);
+                for (int a = 0; a < MT; a++)
 #pragma unroll
                     for (int t = 0; t < NT; t++)
 #pragma unroll
-                        for (int q = 0; q < P; q++) acc[a][t] = w4_mfma(wi, pc[t][q], acc[a][t]);
+                        for (int r = 0; r < 4; r++) acc[a][t][r] = __builtin_fmaf(part[a][t][r], h.s[g][a][r], acc[a][t][r]);
+            }
+        } else {
+            constexpr int P = DT == GR_DT_F32 ? 3 : 2;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float s[8], zk[8];
+                h.gs[i].get(s);
+#pragma unroll
+                for (int e = 0; e < 8; e++) zk[e] = 1024.f + (float)(((e < 4 ? h.gz[i].x : h.gz[i].y) >> (8 * (e & 3))) & 255u);
+                w4_bf16x8 wi[MT];
+#pragma unroll
+                for (int a = 0; a < MT; a++) wi[a] = w4_ints_bf16(h.w[a][i], zk);
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    float g[8];
+                    w4_bf16x8 pc[P];
+                    h.x[i][t].get(g);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) g[e] *= s[e];
+                    w4_pieces<P>(g, pc);
+#pragma unroll
+                    for (int q = 0; q < P; q++)
+#pragma unroll
+                        for (int a = 0; a < MT; a++) acc[a][t] = w4_mfma(wi[a], pc[q], acc[a][t]);
                 }
             }
         }
+    };
+    int c = wave;
+    for (; c + (D - 1) * nwaves < p.chunks; c += D * nwaves) {
+        Chunk h[D];
+#pragma unroll
+        for (int d = 0; d < D; d++) load(h[d], c + d * nwaves);
+#pragma unroll
+        for (int d = 0; d < D; d++) mul(h[d]);
     }
+    if constexpr (D > 1)
+        for (; c < p.chunks; c += nwaves) {
+            Chunk h;
+            load(h, c);
+            mul(h);
+        }
 
     // [wave][tile][reg][lane]
 #pragma unroll
@@ -257,13 +358,7 @@ __global__ __launch_bounds__(1024) void k_w4_rows(W4Params p) {
         const int src = (((mm >> 4) * NT + (nn >> 4)) * 4 + (mm & 3)) * 64 + ((mm >> 2) & 3) * 16 + (nn & 15);
         float v = 0.f;
         for (int w = 0; w < nwaves; w++) v += w4_red[w * (MT * NT * 256) + src];
-        if constexpr (!GRAD) {
-            if (p.bias) v += p.bias[m];
-            if (p.relu) v = v < 0.f ? 0.f : v;
-        } else if (p.gate) {
-            v = (float)((const T*)p.gate)[n * p.ldg + m] > 0.f ? v : 0.f;
-        }
-        ((T*)p.y)[n * p.ldy + m] = (T)v;
+        ((T*)p.y)[n * p.ldy + m] = w4_finish<DT, GRAD>(p, v, n, m);
     }
 }
 
@@ -291,7 +386,7 @@ struct W4Gemm {
     static_assert(LDS <= 160 * 1024, "LDS");
 };
 
-template <int DT, bool GRAD, int TM, int TN, int WM, int WN, int KS>
+template <int DT, int ST, bool GRAD, int TM, int TN, int WM, int WN, int KS>
 __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
     using G = W4Gemm<DT, GRAD, TM, TN, WM, WN, KS>;
     using P = typename G::P;
@@ -310,31 +405,32 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
 
     // ---- staging: thread's share of the weights (AV packed lanes) and of the activations (XV runs of eight)
     unsigned wreg[G::AV][KS];
-    T xreg[G::XV][8];
-    float zreg[GRAD ? 1 : G::AV][KS];
+    W4Raw<DT> xreg[G::XV];
+    uint8_t zreg[GRAD ? 1 : G::AV][KS];
+    W4Raw<ST> sreg[GRAD ? G::AV : 1][KS];                 // GRAD: scales and zeros run along the steps
+    uint2 szreg[GRAD ? G::AV : 1][KS];
     const T* xrow[G::XV];
     int xk[G::XV];
-    bool xlive[G::XV];
 #pragma unroll
     for (int v = 0; v < G::XV; v++) {
         const int f = tid + v * G::NT, l = f & 63, ts = f >> 6;
         const int64_t n = n0 + ts / KS * 16 + (l & 15);
-        xlive[v] = n < p.N;
-        xrow[v] = (const T*)p.x + (xlive[v] ? n : 0) * p.ldx;
         xk[v] = ts % KS * 32 + (l >> 4) * 8;
+        xrow[v] = (const T*)p.x + (n < p.N ? n : p.N - 1) * p.ldx + xk[v];   // columns beyond the batch: computed, not stored
     }
     size_t grow[G::AV];                                   // GRAD: scales / zeros of the thread's row
+    const unsigned* wsrc[G::AV];
 #pragma unroll
     for (int v = 0; v < G::AV; v++) {
         const int row = m0 + (tid + v * G::NT) / 64 * 16 + lr;
-        grow[v] = (size_t)((row < p.R ? row : p.R - 1) / (p.gsteps * 32)) * p.Mp;
+        grow[v] = GRAD ? (size_t)((row < p.R ? row : p.R - 1) / (p.gsteps * 32)) * p.Mp + lh * 8 : 0;
+        wsrc[v] = (const unsigned*)(p.pack + ((size_t)(m0 / 16 + (tid + v * G::NT) / 64) * p.chunks) * 64 + lane);
     }
     int zg = 0, zrem = 0;                                 // group of the next step to load
     auto load = [&](int s) {
 #pragma unroll
         for (int v = 0; v < G::AV; v++) {
-            const size_t rt = m0 / 16 + (tid + v * G::NT) / 64;
-            const unsigned* src = (const unsigned*)(p.pack + (rt * p.chunks + s * KS / 4) * 64 + lane) + s * KS % 4;
+            const unsigned* src = wsrc[v] + (size_t)(s * KS / 4) * 256 + s * KS % 4;
             if constexpr (KS == 2) {
                 const uint2 d = *(const uint2*)src;
                 wreg[v][0] = d.x; wreg[v][1] = d.y;
@@ -342,47 +438,60 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
                 wreg[v][0] = *src;
             }
         }
-        if constexpr (!GRAD) {
 #pragma unroll
-            for (int i = 0; i < KS; i++) {
+        for (int i = 0; i < KS; i++) {
+            if constexpr (!GRAD) {
 #pragma unroll
                 for (int v = 0; v < G::AV; v++)
-                    zreg[v][i] = p.zeros ? (float)p.zeros[(size_t)zg * p.Mp + m0 + (tid + v * G::NT) / 64 * 16 + lr] : 8.f;
+                    zreg[v][i] = p.zeros ? p.zeros[(size_t)zg * p.Mp + m0 + (tid + v * G::NT) / 64 * 16 + lr] : 8;
                 if (++zrem == p.gsteps) { zrem = 0; if ((s * KS + i + 1) * 32 < p.C) zg++; }
+            } else {
+#pragma unroll
+                for (int v = 0; v < G::AV; v++) {
+                    const size_t mb = grow[v] + (s * KS + i) * 32;
+                    sreg[v][i].load((const typename W4Type<ST>::T*)p.scales + mb);
+                    szreg[v][i] = p.zeros ? *(const uint2*)(p.zeros + mb) : uint2{0x08080808u, 0x08080808u};
+                }
             }
         }
+        if ((s + 1) * KS * 32 <= p.C) {
 #pragma unroll
-        for (int v = 0; v < G::XV; v++) w4_load8<DT>(xrow[v], s * KS * 32 + xk[v], p.C, xlive[v], p.xvec != 0, xreg[v]);
+            for (int v = 0; v < G::XV; v++) xreg[v].load(xrow[v] + s * KS * 32);
+        } else {
+#pragma unroll
+            for (int v = 0; v < G::XV; v++) xreg[v].load_part(xrow[v] + s * KS * 32, p.C - s * KS * 32 - xk[v]);
+        }
     };
-    auto store = [&](int s, w4_u32x4* buf) {
+    union Frag { w4_u32x4 u; w4_bf16x8 b; w4_f16x8 h; };
+    auto store = [&](w4_u32x4* buf) {
 #pragma unroll
         for (int v = 0; v < G::AV; v++) {
             const int rt = (tid + v * G::NT) / 64;
 #pragma unroll
             for (int i = 0; i < KS; i++) {
                 w4_u32x4* dst = buf + (rt * KS + i) * 64 + lane;
+                Frag c;
                 if constexpr (F16OP) {
-                    union { w4_f16x8 h; w4_u32x4 u; } c;
-                    c.h = w4_ints_f16(wreg[v][i], zreg[v][i]);
+                    c.h = w4_ints_f16(wreg[v][i], 1024.f + (float)zreg[v][i]);
                     dst[0] = c.u;
                 } else if constexpr (!GRAD) {
-                    union { w4_bf16x8 h; w4_u32x4 u; } c;
-                    c.h = w4_ints_bf16(wreg[v][i], zreg[v][i]);
+                    c.b = w4_ints_bf16(wreg[v][i], 1024.f + (float)zreg[v][i]);
                     dst[0] = c.u;
                 } else {
-                    const size_t mb = grow[v] + s * KS * 32 + i * 32 + lh * 8;
-                    float f[8];
+                    float f[8], sc[8];
+                    sreg[v][i].get(sc);
 #pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const int q = (int)(wreg[v][i] >> (4 * ((e >> 1) + 4 * (e & 1)))) & 15;
-                        f[e] = ((float)q - (p.zeros ? (float)p.zeros[mb + e] : 8.f)) * w4_scale(p.scales, p.st, mb + e);
+                    for (int q = 0; q < 4; q++) {
+                        const unsigned zz = (q < 2 ? szreg[v][i].x : szreg[v][i].y) >> (16 * (q & 1));
+                        w4_ints_f32(wreg[v][i], q, 1024.f + (float)(zz & 255u), 1024.f + (float)(zz >> 8 & 255u), f[2 * q], f[2 * q + 1]);
+                        f[2 * q] *= sc[2 * q];
+                        f[2 * q + 1] *= sc[2 * q + 1];
                     }
                     w4_bf16x8 pc[P::W];
                     w4_pieces<P::W>(f, pc);
 #pragma unroll
                     for (int q = 0; q < P::W; q++) {
-                        union { w4_bf16x8 h; w4_u32x4 u; } c;
-                        c.h = pc[q];
+                        c.b = pc[q];
                         dst[q * G::A_ONE] = c.u;
                     }
                 }
@@ -392,20 +501,16 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
         for (int v = 0; v < G::XV; v++) {
             w4_u32x4* dst = buf + P::W * G::A_ONE + tid + v * G::NT;
             if constexpr (P::X == 1) {
-                union { T t[8]; w4_u32x4 u; } c;
-#pragma unroll
-                for (int e = 0; e < 8; e++) c.t[e] = xreg[v][e];
-                dst[0] = c.u;
+                dst[0] = xreg[v].q[0];
             } else {
                 float f[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) f[e] = (float)xreg[v][e];
+                xreg[v].get(f);
                 w4_bf16x8 pc[P::X];
                 w4_pieces<P::X>(f, pc);
 #pragma unroll
                 for (int q = 0; q < P::X; q++) {
-                    union { w4_bf16x8 h; w4_u32x4 u; } c;
-                    c.h = pc[q];
+                    Frag c;
+                    c.b = pc[q];
                     dst[q * G::X_ONE] = c.u;
                 }
             }
@@ -418,7 +523,6 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
 #pragma unroll
         for (int j = 0; j < TN; j++) acc[i][j] = w4_f32x4{0.f, 0.f, 0.f, 0.f};
     const w4_f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
-    union Frag { w4_u32x4 u; w4_bf16x8 b; w4_f16x8 h; };
     int cg = 0, crem = 0;                                 // group of the step being multiplied
     auto step = [&](const w4_u32x4* buf, int i, bool last) {
         Frag a[P::W][TM], x[P::X][TN];
@@ -447,14 +551,9 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
                 }
         } else {
             const bool flush = crem + 1 == p.gsteps || last;
-            float sc[TM][4];
-            if (flush) {
+            W4Scale4<ST> sc[TM];
 #pragma unroll
-                for (int t = 0; t < TM; t++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        sc[t][r] = w4_scale(p.scales, p.st, (size_t)cg * p.Mp + m0 + (wm * TM + t) * 16 + lh * 4 + r);
-            }
+            for (int t = 0; t < TM; t++) sc[t].load(p.scales, (size_t)cg * p.Mp + m0 + (wm * TM + t) * 16 + lh * 4);
             if (crem == 0) {
 #pragma unroll
                 for (int t = 0; t < TM; t++)
@@ -487,12 +586,12 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
     };
 
     load(0);
-    store(0, w4_lds);
+    store(w4_lds);
     if (nstages > 1) load(1);
     __syncthreads();
     for (int s = 0; s < nstages; s++) {
         if (s + 1 < nstages) {
-            store(s + 1, w4_lds + ((s + 1) & 1) * G::SLOTS);
+            store(w4_lds + ((s + 1) & 1) * G::SLOTS);
             if (s + 2 < nstages) load(s + 2);
         }
         const w4_u32x4* buf = w4_lds + (s & 1) * G::SLOTS;
@@ -512,27 +611,69 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
 #pragma unroll
         for (int t = 0; t < TM; t++) {
             const int m = m0 + (wm * TM + t) * 16 + lh * 4;
-            float v[4];
+            T v[4];
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                v[r] = acc[t][u][r];
-                if (m + r >= p.R) continue;
-                if constexpr (!GRAD) {
-                    if (p.bias) v[r] += p.bias[m + r];
-                    if (p.relu) v[r] = v[r] < 0.f ? 0.f : v[r];
-                } else if (p.gate) {
-                    v[r] = (float)((const T*)p.gate)[n * p.ldg + m + r] > 0.f ? v[r] : 0.f;
-                }
-            }
+            for (int r = 0; r < 4; r++) v[r] = m + r < p.R ? w4_finish<DT, GRAD>(p, acc[t][u][r], n, m + r) : (T)0.f;
             T* dst = (T*)p.y + n * p.ldy + m;
             if (vec && m + 4 <= p.R) {
-                struct alignas(4 * sizeof(T)) T4 { T t[4]; } o = {{(T)v[0], (T)v[1], (T)v[2], (T)v[3]}};
+                struct alignas(4 * sizeof(T)) T4 { T t[4]; } o = {{v[0], v[1], v[2], v[3]}};
                 *(T4*)dst = o;
             } else {
 #pragma unroll
                 for (int r = 0; r < 4; r++)
-                    if (m + r < p.R) dst[r] = (T)v[r];
+                    if (m + r < p.R) dst[r] = v[r];
             }
         }
     }
 }
+
+// ---------------------------------------------------------------------------------------------
+// launchers (one translation unit per activation type: w4_f32.hip, w4_bf16.hip, w4_f16.hip)
+// ---------------------------------------------------------------------------------------------
+hipError_t w4_launch_f32(const W4Params&, int scale_type, bool grad, hipStream_t);
+hipError_t w4_launch_bf16(const W4Params&, int scale_type, bool grad, hipStream_t);
+hipError_t w4_launch_f16(const W4Params&, int scale_type, bool grad, hipStream_t);
+
+#ifdef W4_KERNELS
+template <int DT, int ST, int NT, int GS, bool GRAD>
+static hipError_t launch_rows(const W4Params& p, hipStream_t st) {
+    constexpr int MT = GRAD ? 2 : 1;
+    constexpr int D = DT == GR_DT_F32 || NT > 1 || GRAD ? 1 : 2;
+    const int64_t blocks = (int64_t)((p.R + 16 * MT - 1) / (16 * MT)) * ((p.N + 16 * NT - 1) / (16 * NT));
+    int waves = blocks >= 2048 ? 4 : blocks >= 512 ? 8 : w4_rows_waves(NT, GRAD);
+    if (waves > p.chunks) waves = p.chunks;
+    hipLaunchKernelGGL((k_w4_rows<DT, ST, NT, MT, GS, D, GRAD>), dim3((unsigned)blocks), dim3(waves * 64), (size_t)waves * MT * NT * 1024, st, p);
+    return hipGetLastError();
+}
+template <int DT, int ST, int NT, bool GRAD>
+static hipError_t launch_rows(const W4Params& p, hipStream_t st) {
+    if constexpr (GRAD) return launch_rows<DT, ST, NT, 1, true>(p, st);
+    else if (p.gsteps % 4 == 0) return launch_rows<DT, ST, NT, 1, false>(p, st);
+    else if (p.gsteps % 2 == 0) return launch_rows<DT, ST, NT, 2, false>(p, st);
+    else return launch_rows<DT, ST, NT, 4, false>(p, st);
+}
+template <int DT, int ST, bool GRAD, int TM, int TN, int WM, int WN, int KS>
+static hipError_t launch_gemm(const W4Params& p, hipStream_t st) {
+    using G = W4Gemm<DT, GRAD, TM, TN, WM, WN, KS>;
+    auto kern = &k_w4_gemm<DT, ST, GRAD, TM, TN, WM, WN, KS>;
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, G::LDS);
+    if (e != hipSuccess) return e;
+    const int64_t blocks = (int64_t)((p.R + G::BM - 1) / G::BM) * ((p.N + G::BN - 1) / G::BN);
+    hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(G::NT), G::LDS, st, p);
+    return hipGetLastError();
+}
+template <int DT, int ST, bool GRAD>
+static hipError_t launch_typed(const W4Params& p, hipStream_t st) {
+    if (p.N <= 16) return launch_rows<DT, ST, 1, GRAD>(p, st);
+    if (p.N <= 200) return launch_rows<DT, ST, 2, GRAD>(p, st);
+    if constexpr (GRAD && DT == GR_DT_F32) return launch_gemm<DT, ST, GRAD, 4, 2, 2, 4, 1>(p, st);
+    else if constexpr (DT == GR_DT_F32 || (GRAD && DT == GR_DT_F16)) return launch_gemm<DT, ST, GRAD, 4, 2, 2, 4, 2>(p, st);
+    else return launch_gemm<DT, ST, GRAD, 4, 4, 2, 4, 2>(p, st);
+}
+template <int DT>
+static hipError_t launch_any(const W4Params& p, int scale_type, bool grad, hipStream_t st) {
+    if (scale_type == GR_DT_F32) return grad ? launch_typed<DT, GR_DT_F32, true>(p, st) : launch_typed<DT, GR_DT_F32, false>(p, st);
+    if (scale_type == GR_DT_BF16) return grad ? launch_typed<DT, GR_DT_BF16, true>(p, st) : launch_typed<DT, GR_DT_BF16, false>(p, st);
+    return grad ? launch_typed<DT, GR_DT_F16, true>(p, st) : launch_typed<DT, GR_DT_F16, false>(p, st);
+}
+#endif

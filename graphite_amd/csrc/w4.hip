@@ -112,32 +112,10 @@ extern "C" int gr_w4_create(gr_ctx* ctx, const uint8_t* q, int64_t ldq, const vo
     return GR_OK;
 }
 
-template <int DT, int NT, bool GRAD>
-static void launch_rows(const W4Params& p, hipStream_t st) {
-    constexpr int MT = GRAD ? 2 : 1;
-    const int64_t blocks = (int64_t)((p.R + 16 * MT - 1) / (16 * MT)) * ((p.N + 16 * NT - 1) / (16 * NT));
-    int waves = blocks >= 2048 ? 4 : blocks >= 512 ? 8 : 16;
-    if (waves > p.chunks) waves = p.chunks;
-    hipLaunchKernelGGL((k_w4_rows<DT, NT, MT, GRAD>), dim3((unsigned)blocks), dim3(waves * 64), (size_t)waves * MT * NT * 1024, st, p);
-}
-template <int DT, bool GRAD, int TM, int TN, int WM, int WN, int KS>
-static hipError_t launch_gemm(const W4Params& p, hipStream_t st) {
-    using G = W4Gemm<DT, GRAD, TM, TN, WM, WN, KS>;
-    auto kern = &k_w4_gemm<DT, GRAD, TM, TN, WM, WN, KS>;
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, G::LDS);
-    if (e != hipSuccess) return e;
-    const int64_t blocks = (int64_t)((p.R + G::BM - 1) / G::BM) * ((p.N + G::BN - 1) / G::BN);
-    hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(G::NT), G::LDS, st, p);
-    return hipGetLastError();
-}
-template <int DT, bool GRAD>
-static hipError_t launch_any(const W4Params& p, hipStream_t st) {
-    if (p.N <= 16) launch_rows<DT, 1, GRAD>(p, st);
-    else if (p.N <= 200) launch_rows<DT, 2, GRAD>(p, st);
-    else if constexpr (GRAD && DT == GR_DT_F32) return launch_gemm<DT, GRAD, 4, 2, 2, 4, 1>(p, st);
-    else if constexpr (DT == GR_DT_F32 || (GRAD && DT == GR_DT_F16)) return launch_gemm<DT, GRAD, 4, 2, 2, 4, 2>(p, st);
-    else return launch_gemm<DT, GRAD, 4, 4, 2, 4, 2>(p, st);
-    return hipGetLastError();
+static hipError_t w4_launch(const W4Params& p, int dt, int scale_type, bool grad, hipStream_t st) {
+    if (dt == GR_DT_F32) return w4_launch_f32(p, scale_type, grad, st);
+    if (dt == GR_DT_BF16) return w4_launch_bf16(p, scale_type, grad, st);
+    return w4_launch_f16(p, scale_type, grad, st);
 }
 
 static int w4_run(gr_ctx* ctx, const gr_w4* w, const char* who, bool grad, const void* x, int dt, int64_t N, int64_t ldx, const void* gate,
@@ -157,24 +135,15 @@ static int w4_run(gr_ctx* ctx, const gr_w4* w, const char* who, bool grad, const
     if (((uintptr_t)x | (uintptr_t)y | (uintptr_t)gate) % es) return gr_fail(ctx, GR_EINVAL, "%s: misaligned tensor", who);
     if ((int64_t)((p.R + 15) / 16) * ((N + 15) / 16) > INT_MAX) return gr_fail(ctx, GR_EINVAL, "%s: batch too large", who);
     p.pack = grad ? w->packT : w->pack;
-    p.scales = w->scales; p.zeros = w->zeros; p.st = w->st; p.Mp = w->Mp;
+    p.scales = w->scales; p.zeros = w->zeros; p.Mp = w->Mp;
     p.chunks = (grad ? w->Mp : w->Kp) / W4_CHUNK;
     p.gsteps = w->group / 32;
     p.x = x; p.y = y; p.bias = w->bias; p.gate = gate;
     p.N = N; p.ldx = ldx; p.ldy = ldy; p.ldg = ldg; p.relu = relu;
-    p.xvec = ((uintptr_t)x % 16 == 0) && (ldx * (int64_t)es % 16 == 0);
     const double fl = 2.0 * (double)N * w->M * w->K;
     const double by = (double)w->M * w->K / 2 + (double)w->M * w->G * (dt_size(w->st) + (w->zeros ? 1 : 0)) + (double)N * (w->M + w->K) * es;
     ProfScope ps(ctx, grad ? "k_w4_grad" : "k_w4_forward", st, fl, by);
-    hipError_t e;
-    switch (dt * 2 + (grad ? 1 : 0)) {
-        case GR_DT_F32 * 2: e = launch_any<GR_DT_F32, false>(p, st); break;
-        case GR_DT_F32 * 2 + 1: e = launch_any<GR_DT_F32, true>(p, st); break;
-        case GR_DT_BF16 * 2: e = launch_any<GR_DT_BF16, false>(p, st); break;
-        case GR_DT_BF16 * 2 + 1: e = launch_any<GR_DT_BF16, true>(p, st); break;
-        case GR_DT_F16 * 2: e = launch_any<GR_DT_F16, false>(p, st); break;
-        default: e = launch_any<GR_DT_F16, true>(p, st); break;
-    }
+    const hipError_t e = w4_launch(p, dt, w->st, grad, st);
     GR_HIP(ctx, e);
     return GR_OK;
 }

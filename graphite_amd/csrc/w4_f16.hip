@@ -1,0 +1,7 @@
+// w4_f16.hip -- the 4-bit linear kernels (w4.h) for float16 activations.
+#define W4_KERNELS
+#include "w4.h"
+
+hipError_t w4_launch_f16(const W4Params& p, int scale_type, bool grad, hipStream_t st) {
+    return launch_any<GR_DT_F16>(p, scale_type, grad, st);
+}
