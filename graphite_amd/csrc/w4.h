@@ -186,7 +186,7 @@ __device__ __forceinline__ typename W4Type<DT>::T w4_finish(const W4Params& p, f
 // chunks at a time (all their loads are issued before the first is used), and their sums meet in LDS, in wave order.
 // Forward: GS = groups of a chunk (1, 2 or 4; 4 also where a border falls on any step).
 // ---------------------------------------------------------------------------------------------
-constexpr int w4_rows_waves(int nt, bool grad) { return nt > 1 && grad ? 8 : 16; }      // the most a workgroup may have
+constexpr int w4_rows_waves(int nt, bool) { return nt > 1 ? 8 : 16; }      // the most a workgroup may have
 template <int DT, int ST, int NT, int MT, int GS, int D, bool GRAD>
 __global__ __launch_bounds__(w4_rows_waves(NT, GRAD) * 64) void k_w4_rows(W4Params p) {
     typedef typename W4Type<DT>::T T;
@@ -379,11 +379,13 @@ struct W4Gemm {
     using P = W4Pieces<DT, GRAD>;
     static constexpr int NT = WM * WN * 64, BM = WM * TM * 16, BN = WN * TN * 16;
     static constexpr int A_ONE = BM / 16 * KS * 64, X_ONE = BN / 16 * KS * 64;      // 16-byte slots of one piece
-    static constexpr int SLOTS = A_ONE * P::W + X_ONE * P::X;
+    static constexpr int SC = GRAD ? 0 : KS * BM;       // forward: f32 scales of the stage's steps, one per row
+    static constexpr int SC0 = A_ONE * P::W + X_ONE * P::X, SLOTS = SC0 + SC / 4;
     static constexpr int LDS = 2 * SLOTS * 16;
     static constexpr int AV = BM / 16 * 64 / NT, XV = X_ONE / NT;
     static_assert(BM / 16 * 64 % NT == 0 && X_ONE % NT == 0, "stage loads must divide evenly");
     static_assert(LDS <= 160 * 1024, "LDS");
+    static_assert(SC <= NT, "one scale per thread and stage");
 };
 
 template <int DT, int ST, bool GRAD, int TM, int TN, int WM, int WN, int KS>
@@ -426,6 +428,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
         grow[v] = GRAD ? (size_t)((row < p.R ? row : p.R - 1) / (p.gsteps * 32)) * p.Mp + lh * 8 : 0;
         wsrc[v] = (const unsigned*)(p.pack + ((size_t)(m0 / 16 + (tid + v * G::NT) / 64) * p.chunks) * 64 + lane);
     }
+    typename W4Type<ST>::T screg = 0.f;                   // forward: scale of row m0 + tid % BM, step tid / BM of the stage
     int zg = 0, zrem = 0;                                 // group of the next step to load
     auto load = [&](int s) {
 #pragma unroll
@@ -444,6 +447,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
 #pragma unroll
                 for (int v = 0; v < G::AV; v++)
                     zreg[v][i] = p.zeros ? p.zeros[(size_t)zg * p.Mp + m0 + (tid + v * G::NT) / 64 * 16 + lr] : 8;
+                if (tid / G::BM == i) screg = ((const typename W4Type<ST>::T*)p.scales)[(size_t)zg * p.Mp + m0 + tid % G::BM];
                 if (++zrem == p.gsteps) { zrem = 0; if ((s * KS + i + 1) * 32 < p.C) zg++; }
             } else {
 #pragma unroll
@@ -497,6 +501,9 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
                 }
             }
         }
+        if constexpr (!GRAD) {
+            if (tid < G::SC) ((float*)(buf + G::SC0))[tid] = (float)screg;
+        }
 #pragma unroll
         for (int v = 0; v < G::XV; v++) {
             w4_u32x4* dst = buf + P::W * G::A_ONE + tid + v * G::NT;
@@ -523,7 +530,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
 #pragma unroll
         for (int j = 0; j < TN; j++) acc[i][j] = w4_f32x4{0.f, 0.f, 0.f, 0.f};
     const w4_f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
-    int cg = 0, crem = 0;                                 // group of the step being multiplied
+    int crem = 0;                                         // steps of the group multiplied so far
     auto step = [&](const w4_u32x4* buf, int i, bool last) {
         Frag a[P::W][TM], x[P::X][TN];
 #pragma unroll
@@ -551,9 +558,12 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
                 }
         } else {
             const bool flush = crem + 1 == p.gsteps || last;
-            W4Scale4<ST> sc[TM];
+            // scales come through LDS: a wait on a global load here would wait for the next stage's loads as well
+            w4_f32x4 sc[TM];
+            if (flush) {
 #pragma unroll
-            for (int t = 0; t < TM; t++) sc[t].load(p.scales, (size_t)cg * p.Mp + m0 + (wm * TM + t) * 16 + lh * 4);
+                for (int t = 0; t < TM; t++) sc[t] = *(const w4_f32x4*)((const float*)(buf + G::SC0) + i * G::BM + (wm * TM + t) * 16 + lh * 4);
+            }
             if (crem == 0) {
 #pragma unroll
                 for (int t = 0; t < TM; t++)
@@ -580,7 +590,6 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
 #pragma unroll
                         for (int r = 0; r < 4; r++) acc[t][u][r] = __builtin_fmaf(part[t][u][r], sc[t][r], acc[t][u][r]);
                 crem = 0;
-                cg++;
             }
         }
     };
