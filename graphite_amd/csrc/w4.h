@@ -31,8 +31,8 @@ constexpr int W4_CHUNK = 128;         // contraction steps of a tile
 struct W4Params {
     const w4_u32x4* pack;    // [row tiles][chunks][64]
     const void* scales;      // [groups][Mp], type ST of the kernel
-    const uint8_t* zeros;    // [groups][Mp], or null: 8 everywhere
-    int Mp;                  // padded out_features
+    const uint8_t* zeros;    // [groups][Mp]; zstride 0: one row of eights for every group
+    int Mp, zstride;         // padded out_features, and what zeros advance by per group (Mp or 0)
     int chunks;              // of the contraction
     int C, R;                // contraction length, output columns (true sizes)
     int gsteps;              // group / 32
@@ -57,8 +57,10 @@ __device__ __forceinline__ unsigned w4_pack_hi(float a, float b) {       // high
 __device__ __forceinline__ void w4_ints_f32(unsigned w, int p, float z0, float z1, float& a, float& b) {
     union { unsigned u; w4_f16x2 h; } c;
     c.u = ((w >> (4 * p)) & 0x000f000fu) | 0x64006400u;
-    a = __builtin_fmaf((float)c.h[0], 1.f, -z0);
-    b = __builtin_fmaf((float)c.h[1], 1.f, -z1);
+    float one = 1.f;
+    asm("" : "+s"(one));                                 // a factor the compiler cannot drop: it would convert and subtract in two steps
+    a = __builtin_fmaf((float)c.h[0], one, -z0);
+    b = __builtin_fmaf((float)c.h[1], one, -z1);
 }
 // eight nibbles - z as bf16 (exact: |v| <= 15); zk = 1024 + z
 __device__ __forceinline__ w4_bf16x8 w4_ints_bf16(unsigned w, const float (&zk)[8]) {
@@ -202,7 +204,8 @@ __global__ __launch_bounds__(w4_rows_waves(NT, GRAD) * 64) void k_w4_rows(W4Para
         const int64_t n = n0 + t * 16 + lr;
         xrow[t] = (const T*)p.x + (n < p.N ? n : p.N - 1) * p.ldx + lh * 8;      // columns beyond the batch: computed, not stored
     }
-    const size_t grow = GRAD ? (size_t)((rt0 >> 1) / p.gsteps) * p.Mp : 0;        // group of the rows (MT is 1 or 2)
+    const size_t grow = GRAD ? (size_t)((rt0 >> 1) / p.gsteps) * p.Mp : 0;        // the rows' one group
+    const size_t zrow = GRAD ? (size_t)((rt0 >> 1) / p.gsteps) * p.zstride : 0;
     w4_f32x4 acc[MT][NT];
 #pragma unroll
     for (int a = 0; a < MT; a++)
@@ -237,11 +240,11 @@ __global__ __launch_bounds__(w4_rows_waves(NT, GRAD) * 64) void k_w4_rows(W4Para
             for (int g = 0; g < GS; g++) {
                 int step = c * 4 + g * (4 / GS);
                 if (step * 32 >= p.C) step = c * 4;                               // beyond the row: x is 0 there
-                const size_t row = (size_t)(step / p.gsteps) * p.Mp + (size_t)rt0 * 16;
+                const size_t g_ = (size_t)(step / p.gsteps), row = g_ * p.Mp + (size_t)rt0 * 16, zr = g_ * p.zstride + (size_t)rt0 * 16;
 #pragma unroll
                 for (int a = 0; a < MT; a++) {
                     h.s[g][a].load(p.scales, row + a * 16 + lh * 4);
-                    h.z[g][a] = p.zeros ? p.zeros[row + a * 16 + lr] : 8;
+                    h.z[g][a] = p.zeros[zr + a * 16 + lr];
                 }
             }
         } else {
@@ -249,7 +252,7 @@ __global__ __launch_bounds__(w4_rows_waves(NT, GRAD) * 64) void k_w4_rows(W4Para
             for (int i = 0; i < 4; i++) {
                 const size_t mb = grow + kb + i * 32 + lh * 8;
                 h.gs[i].load((const typename W4Type<ST>::T*)p.scales + mb);
-                h.gz[i] = p.zeros ? *(const uint2*)(p.zeros + mb) : uint2{0x08080808u, 0x08080808u};
+                h.gz[i] = *(const uint2*)(p.zeros + zrow + kb + i * 32 + lh * 8);
             }
         }
     };
@@ -367,25 +370,27 @@ __global__ __launch_bounds__(w4_rows_waves(NT, GRAD) * 64) void k_w4_rows(W4Para
 // KS * 32 contraction steps is turned into matrix-instruction operands ONCE per workgroup (4-bit weights to integers, f32
 // activations to pieces) on its way global -> registers -> LDS.  LDS holds operands in fragment order ([tile][step][64 lanes]
 // [16 bytes], the order the packed weights already have), so every LDS access is 64 lanes x 16 consecutive bytes.
-// Two LDS buffers, one barrier per stage, global loads one stage ahead.
+// Three LDS buffers, one barrier per stage: while a stage is multiplied, the next one's first operands are already read and
+// the one after is written, from registers that global memory filled a stage earlier.
 // ---------------------------------------------------------------------------------------------
 template <int DT, bool GRAD> struct W4Pieces {          // pieces of the weights and of the activations
     static constexpr int W = !GRAD ? 1 : DT == GR_DT_F32 ? 3 : 2;
     static constexpr int X = DT == GR_DT_F32 ? 3 : GRAD && DT == GR_DT_F16 ? 2 : 1;
     static constexpr int TOP = W > X ? W : X;           // products i, j with i + j < TOP count
+    static constexpr int PROD = !GRAD ? X : DT == GR_DT_F32 ? 6 : DT == GR_DT_F16 ? 3 : 2;
 };
 template <int DT, bool GRAD, int TM, int TN, int WM, int WN, int KS>
 struct W4Gemm {
     using P = W4Pieces<DT, GRAD>;
     static constexpr int NT = WM * WN * 64, BM = WM * TM * 16, BN = WN * TN * 16;
     static constexpr int A_ONE = BM / 16 * KS * 64, X_ONE = BN / 16 * KS * 64;      // 16-byte slots of one piece
-    static constexpr int SC = GRAD ? 0 : KS * BM;       // forward: f32 scales of the stage's steps, one per row
+    static constexpr int SC = GRAD ? 0 : NT;            // forward: f32 scales of the stage's steps, one per row (KS * BM of them, repeated)
     static constexpr int SC0 = A_ONE * P::W + X_ONE * P::X, SLOTS = SC0 + SC / 4;
-    static constexpr int LDS = 2 * SLOTS * 16;
+    static constexpr int LDS = 3 * SLOTS * 16;
     static constexpr int AV = BM / 16 * 64 / NT, XV = X_ONE / NT;
     static_assert(BM / 16 * 64 % NT == 0 && X_ONE % NT == 0, "stage loads must divide evenly");
     static_assert(LDS <= 160 * 1024, "LDS");
-    static_assert(SC <= NT, "one scale per thread and stage");
+    static_assert(GRAD || NT % (KS * BM) == 0, "one scale per thread and stage");
 };
 
 template <int DT, int ST, bool GRAD, int TM, int TN, int WM, int WN, int KS>
@@ -420,17 +425,20 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
         xk[v] = ts % KS * 32 + (l >> 4) * 8;
         xrow[v] = (const T*)p.x + (n < p.N ? n : p.N - 1) * p.ldx + xk[v];   // columns beyond the batch: computed, not stored
     }
-    size_t grow[G::AV];                                   // GRAD: scales / zeros of the thread's row
+    size_t grow[G::AV], zrow[G::AV];                      // GRAD: scales / zeros of the thread's row
     const unsigned* wsrc[G::AV];
 #pragma unroll
     for (int v = 0; v < G::AV; v++) {
         const int row = m0 + (tid + v * G::NT) / 64 * 16 + lr;
-        grow[v] = GRAD ? (size_t)((row < p.R ? row : p.R - 1) / (p.gsteps * 32)) * p.Mp + lh * 8 : 0;
+        const size_t g_ = GRAD ? (size_t)((row < p.R ? row : p.R - 1) / (p.gsteps * 32)) : 0;
+        grow[v] = g_ * p.Mp + lh * 8;
+        zrow[v] = g_ * p.zstride + lh * 8;
         wsrc[v] = (const unsigned*)(p.pack + ((size_t)(m0 / 16 + (tid + v * G::NT) / 64) * p.chunks) * 64 + lane);
     }
-    typename W4Type<ST>::T screg = 0.f;                   // forward: scale of row m0 + tid % BM, step tid / BM of the stage
+    typename W4Type<ST>::T screg;                         // forward: scale of row m0 + tid % BM, step tid / BM % KS of the stage
+    const int sstep = __builtin_amdgcn_readfirstlane(tid / G::BM % KS);
     int zg = 0, zrem = 0;                                 // group of the next step to load
-    auto load = [&](int s) {
+    auto load_w = [&](int s) {                            // weights with their scales and zeros
 #pragma unroll
         for (int v = 0; v < G::AV; v++) {
             const unsigned* src = wsrc[v] + (size_t)(s * KS / 4) * 256 + s * KS % 4;
@@ -441,23 +449,30 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
                 wreg[v][0] = *src;
             }
         }
+        int sg = zg;
 #pragma unroll
         for (int i = 0; i < KS; i++) {
             if constexpr (!GRAD) {
 #pragma unroll
                 for (int v = 0; v < G::AV; v++)
-                    zreg[v][i] = p.zeros ? p.zeros[(size_t)zg * p.Mp + m0 + (tid + v * G::NT) / 64 * 16 + lr] : 8;
-                if (tid / G::BM == i) screg = ((const typename W4Type<ST>::T*)p.scales)[(size_t)zg * p.Mp + m0 + tid % G::BM];
-                if (++zrem == p.gsteps) { zrem = 0; if ((s * KS + i + 1) * 32 < p.C) zg++; }
+                    zreg[v][i] = p.zeros[(size_t)zg * p.zstride + m0 + (tid + v * G::NT) / 64 * 16 + lr];
+                sg = sstep == i ? zg : sg;
+                zrem++;
+                const bool end = zrem == p.gsteps;        // the next step, if there is one, begins a group
+                zg += end && (s * KS + i + 1) * 32 < p.C ? 1 : 0;
+                zrem = end ? 0 : zrem;
             } else {
 #pragma unroll
                 for (int v = 0; v < G::AV; v++) {
-                    const size_t mb = grow[v] + (s * KS + i) * 32;
-                    sreg[v][i].load((const typename W4Type<ST>::T*)p.scales + mb);
-                    szreg[v][i] = p.zeros ? *(const uint2*)(p.zeros + mb) : uint2{0x08080808u, 0x08080808u};
+                    sreg[v][i].load((const typename W4Type<ST>::T*)p.scales + grow[v] + (s * KS + i) * 32);
+                    szreg[v][i] = *(const uint2*)(p.zeros + zrow[v] + (s * KS + i) * 32);
                 }
             }
         }
+        if constexpr (!GRAD) screg = ((const typename W4Type<ST>::T*)p.scales)[(size_t)sg * p.Mp + m0 + tid % G::BM];
+    };
+    auto load = [&](int s) {
+        load_w(s);
         if ((s + 1) * KS * 32 <= p.C) {
 #pragma unroll
             for (int v = 0; v < G::XV; v++) xreg[v].load(xrow[v] + s * KS * 32);
@@ -467,61 +482,62 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
         }
     };
     union Frag { w4_u32x4 u; w4_bf16x8 b; w4_f16x8 h; };
+    auto store_w = [&](w4_u32x4* buf, int v, int i) {
+        w4_u32x4* dst = buf + ((tid + v * G::NT) / 64 * KS + i) * 64 + lane;
+        Frag c;
+        if constexpr (F16OP) {
+            c.h = w4_ints_f16(wreg[v][i], 1024.f + (float)zreg[v][i]);
+            dst[0] = c.u;
+        } else if constexpr (!GRAD) {
+            c.b = w4_ints_bf16(wreg[v][i], 1024.f + (float)zreg[v][i]);
+            dst[0] = c.u;
+        } else {
+            float f[8], sc[8];
+            sreg[v][i].get(sc);
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const unsigned zz = (q < 2 ? szreg[v][i].x : szreg[v][i].y) >> (16 * (q & 1));
+                w4_ints_f32(wreg[v][i], q, 1024.f + (float)(zz & 255u), 1024.f + (float)(zz >> 8 & 255u), f[2 * q], f[2 * q + 1]);
+                f[2 * q] *= sc[2 * q];
+                f[2 * q + 1] *= sc[2 * q + 1];
+            }
+            w4_bf16x8 pc[P::W];
+            w4_pieces<P::W>(f, pc);
+#pragma unroll
+            for (int q = 0; q < P::W; q++) {
+                c.b = pc[q];
+                dst[q * G::A_ONE] = c.u;
+            }
+        }
+    };
+    auto store_x = [&](w4_u32x4* buf, int v) {
+        w4_u32x4* dst = buf + P::W * G::A_ONE + tid + v * G::NT;
+        if constexpr (P::X == 1) {
+            dst[0] = xreg[v].q[0];
+        } else {
+            float f[8];
+            xreg[v].get(f);
+            w4_bf16x8 pc[P::X];
+            w4_pieces<P::X>(f, pc);
+#pragma unroll
+            for (int q = 0; q < P::X; q++) {
+                Frag c;
+                c.b = pc[q];
+                dst[q * G::X_ONE] = c.u;
+            }
+        }
+    };
+    auto store_sc = [&](w4_u32x4* buf) {
+        if constexpr (!GRAD) ((float*)(buf + G::SC0))[tid] = (float)screg;
+    };
     auto store = [&](w4_u32x4* buf) {
 #pragma unroll
-        for (int v = 0; v < G::AV; v++) {
-            const int rt = (tid + v * G::NT) / 64;
+        for (int v = 0; v < G::AV; v++)
 #pragma unroll
-            for (int i = 0; i < KS; i++) {
-                w4_u32x4* dst = buf + (rt * KS + i) * 64 + lane;
-                Frag c;
-                if constexpr (F16OP) {
-                    c.h = w4_ints_f16(wreg[v][i], 1024.f + (float)zreg[v][i]);
-                    dst[0] = c.u;
-                } else if constexpr (!GRAD) {
-                    c.b = w4_ints_bf16(wreg[v][i], 1024.f + (float)zreg[v][i]);
-                    dst[0] = c.u;
-                } else {
-                    float f[8], sc[8];
-                    sreg[v][i].get(sc);
+            for (int i = 0; i < KS; i++) store_w(buf, v, i);
+        store_sc(buf);
 #pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        const unsigned zz = (q < 2 ? szreg[v][i].x : szreg[v][i].y) >> (16 * (q & 1));
-                        w4_ints_f32(wreg[v][i], q, 1024.f + (float)(zz & 255u), 1024.f + (float)(zz >> 8 & 255u), f[2 * q], f[2 * q + 1]);
-                        f[2 * q] *= sc[2 * q];
-                        f[2 * q + 1] *= sc[2 * q + 1];
-                    }
-                    w4_bf16x8 pc[P::W];
-                    w4_pieces<P::W>(f, pc);
-#pragma unroll
-                    for (int q = 0; q < P::W; q++) {
-                        c.b = pc[q];
-                        dst[q * G::A_ONE] = c.u;
-                    }
-                }
-            }
-        }
-        if constexpr (!GRAD) {
-            if (tid < G::SC) ((float*)(buf + G::SC0))[tid] = (float)screg;
-        }
-#pragma unroll
-        for (int v = 0; v < G::XV; v++) {
-            w4_u32x4* dst = buf + P::W * G::A_ONE + tid + v * G::NT;
-            if constexpr (P::X == 1) {
-                dst[0] = xreg[v].q[0];
-            } else {
-                float f[8];
-                xreg[v].get(f);
-                w4_bf16x8 pc[P::X];
-                w4_pieces<P::X>(f, pc);
-#pragma unroll
-                for (int q = 0; q < P::X; q++) {
-                    Frag c;
-                    c.b = pc[q];
-                    dst[q * G::X_ONE] = c.u;
-                }
-            }
-        }
+        for (int v = 0; v < G::XV; v++) store_x(buf, v);
     };
 
     w4_f32x4 acc[TM][TN], part[GRAD ? 1 : TM][GRAD ? 1 : TN];
@@ -531,6 +547,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
         for (int j = 0; j < TN; j++) acc[i][j] = w4_f32x4{0.f, 0.f, 0.f, 0.f};
     const w4_f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
     int crem = 0;                                         // steps of the group multiplied so far
+    bool fresh = true;                                    // none of them is in `part`
     auto step = [&](const w4_u32x4* buf, int i, bool last) {
         Frag a[P::W][TM], x[P::X][TN];
 #pragma unroll
@@ -564,7 +581,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
 #pragma unroll
                 for (int t = 0; t < TM; t++) sc[t] = *(const w4_f32x4*)((const float*)(buf + G::SC0) + i * G::BM + (wm * TM + t) * 16 + lh * 4);
             }
-            if (crem == 0) {
+            if (fresh) {
 #pragma unroll
                 for (int t = 0; t < TM; t++)
 #pragma unroll
@@ -581,7 +598,8 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
                 for (int t = 0; t < TM; t++)
 #pragma unroll
                     for (int u = 0; u < TN; u++) part[t][u] = mul(0, qx, t, u, part[t][u]);
-            crem++;
+            fresh = flush;
+            crem = crem + 1 == p.gsteps ? 0 : crem + 1;
             if (flush) {
 #pragma unroll
                 for (int t = 0; t < TM; t++)
@@ -589,27 +607,204 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
                     for (int u = 0; u < TN; u++)
 #pragma unroll
                         for (int r = 0; r < 4; r++) acc[t][u][r] = __builtin_fmaf(part[t][u][r], sc[t][r], acc[t][u][r]);
-                crem = 0;
             }
         }
     };
 
-    load(0);
-    store(w4_lds);
-    if (nstages > 1) load(1);
-    __syncthreads();
-    for (int s = 0; s < nstages; s++) {
-        if (s + 1 < nstages) {
-            store(w4_lds + ((s + 1) & 1) * G::SLOTS);
-            if (s + 2 < nstages) load(s + 2);
+    // 64 contraction steps without borders: straight-line code.  Its matrix instructions are cut into slices of one row tile
+    // (TN of them), and the staging is dealt out over the slices, where it runs in the matrix unit's shadow.
+    // FIRST: the steps begin a group, FLUSH: they end one.  F holds the operands of the first step.
+    Frag fa[2][P::W][TM], fx[2][P::X][TN];
+    auto read_a = [&](int f, const w4_u32x4* buf, int i) {
+#pragma unroll
+        for (int q = 0; q < P::W; q++)
+#pragma unroll
+            for (int t = 0; t < TM; t++) fa[f][q][t].u = buf[q * G::A_ONE + ((wm * TM + t) * KS + i) * 64 + lane];
+    };
+    auto read_x = [&](int f, const w4_u32x4* buf, int i) {
+#pragma unroll
+        for (int q = 0; q < P::X; q++)
+#pragma unroll
+            for (int t = 0; t < TN; t++) fx[f][q][t].u = buf[P::W * G::A_ONE + q * G::X_ONE + ((wn * TN + t) * KS + i) * 64 + lane];
+    };
+    w4_u32x4 *b0 = w4_lds, *b1 = w4_lds + G::SLOTS, *b2 = w4_lds + 2 * G::SLOTS;      // stages s, s + 1, s + 2
+    auto body = [&]<bool FIRST, bool FLUSH>(int s) {
+        constexpr int STEPS = 2 / KS * KS, NSL = KS * P::PROD * TM, NW = G::AV * KS, ITEMS = NW + 2 + 2 * G::XV;
+        static_assert(STEPS == 2, "");
+        auto mul = [&](int f, int qa, int qx, int t, int u, w4_f32x4 c) {
+            if constexpr (F16OP) return w4_mfma(fa[f][qa][t].h, fx[f][qx][u].h, c);
+            else return w4_mfma(fa[f][qa][t].b, fx[f][qx][u].b, c);
+        };
+        w4_f32x4 sc[GRAD ? 1 : TM];
+        auto flush = [&](int t) {
+#pragma unroll
+            for (int u = 0; u < TN; u++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) acc[t][u][r] = __builtin_fmaf(part[t][u][r], sc[t][r], acc[t][u][r]);
+        };
+        int sl = 0;
+#pragma unroll
+        for (int f = 0; f < 2; f++) {                     // step f; its operands are fa[f], fx[f]
+            const int i = KS == 2 ? f : 0, st = s + (KS == 2 ? 0 : f);      // step of the stage, stage
+            if (KS == 1) sl = 0;
+            auto item = [&](int it) {
+                if (it < NW) store_w(b2, it / KS, it % KS);
+                else if (it == NW) store_sc(b2);
+                else if (it == NW + 1) load_w(st + 3);
+                else if ((it - NW) % 2 == 0) store_x(b2, (it - NW - 2) / 2);
+                else xreg[(it - NW - 2) / 2].load(xrow[(it - NW - 2) / 2] + (st + 3) * KS * 32);
+            };
+            const bool wrap = i == KS - 1;                // the next step is the next stage's first
+            int pr = 0;
+#pragma unroll
+            for (int qa = 0; qa < P::W; qa++)
+#pragma unroll
+                for (int qx = 0; qx < P::X; qx++) {
+                    if (qa + qx >= P::TOP) continue;
+                    pr++;
+#pragma unroll
+                    for (int t = 0; t < TM; t++) {
+#pragma unroll
+                        for (int u = 0; u < TN; u++) {
+                            if constexpr (GRAD) acc[t][u] = mul(f, qa, qx, t, u, acc[t][u]);
+                            else part[t][u] = mul(f, qa, qx, t, u, FIRST && f == 0 && qx == 0 ? zero4 : part[t][u]);
+                        }
+                        if (pr == 1 && t == 0) read_a(1 - f, wrap ? b1 : b0, wrap ? 0 : 1);
+                        if (pr == 1 && t == 1) read_x(1 - f, wrap ? b1 : b0, wrap ? 0 : 1);
+#pragma unroll
+                        for (int it = 0; it < ITEMS; it++)
+                            if (it * NSL / ITEMS == sl) item(it);
+                        if constexpr (!GRAD && FLUSH) {
+                            if (f == 1 && pr == P::PROD) {
+                                sc[t] = *(const w4_f32x4*)((const float*)(b0 + G::SC0) + (KS - 1) * G::BM + (wm * TM + t) * 16 + lh * 4);
+                                if (t > 0) flush(t - 1);
+                            }
+                        }
+                        sl++;
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+            if (wrap) {
+                if constexpr (!GRAD && FLUSH) {
+                    if (f == 1) flush(TM - 1);
+                }
+                __syncthreads();
+                w4_u32x4* t = b0; b0 = b1; b1 = b2; b2 = t;
+            }
         }
-        const w4_u32x4* buf = w4_lds + (s & 1) * G::SLOTS;
+    };
+
+    // The same for 16-bit activations, forward (KS = 2): a row tile's partial sums live for one slice only -- they are scaled and
+    // added after every 64 steps (PERSTEP: 32, for groups that are an odd multiple of that), also inside a group.  Partial sums
+    // held over whole groups would need 64 more registers than the 256 there are.
+    Frag qa[2][KS], qx[2][KS][TN];
+    auto read_qa = [&](const w4_u32x4* buf, int t) {
+#pragma unroll
+        for (int i = 0; i < KS; i++) qa[t & 1][i].u = buf[((wm * TM + t) * KS + i) * 64 + lane];
+    };
+    auto read_qx = [&](int set, const w4_u32x4* buf, int t) {
+#pragma unroll
+        for (int i = 0; i < KS; i++) qx[set][i][t].u = buf[G::A_ONE + ((wn * TN + t) * KS + i) * 64 + lane];
+    };
+    auto body16 = [&]<bool PERSTEP, int SET>(int s) {
+        constexpr int NW = G::AV * KS, ITEMS = NW + 2 + 2 * G::XV;
+        auto item = [&](int it) {
+            if (it < NW) store_w(b2, it / KS, it % KS);
+            else if (it == NW) store_sc(b2);
+            else if (it == NW + 1) load_w(s + 3);
+            else if ((it - NW) % 2 == 0) store_x(b2, (it - NW - 2) / 2);
+            else xreg[(it - NW - 2) / 2].load(xrow[(it - NW - 2) / 2] + (s + 3) * KS * 32);
+        };
+        constexpr int FS = PERSTEP ? KS : 1;               // partial sums a slice leaves behind, one after the other
+        w4_f32x4 ps[2][TN], sc[2];
+        auto flush = [&](int j) {
+#pragma unroll
+            for (int u = 0; u < TN; u++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) acc[j / FS][u][r] = __builtin_fmaf(ps[j & 1][u][r], sc[j & 1][r], acc[j / FS][u][r]);
+        };
+#pragma unroll
+        for (int t = 0; t < TM; t++) {
+            read_qa(t + 1 < TM ? b0 : b1, (t + 1) % TM);
+            if (t < TN) read_qx(1 - SET, b1, t);
+#pragma unroll
+            for (int i = 0; i < KS; i++) {
+                const int j = t * FS + (PERSTEP ? i : 0);
+                if (PERSTEP || i == 0)
+                    sc[j & 1] = *(const w4_f32x4*)((const float*)(b0 + G::SC0) + (PERSTEP ? i : KS - 1) * G::BM + (wm * TM + t) * 16 + lh * 4);
+#pragma unroll
+                for (int u = 0; u < TN; u++) {
+                    const w4_f32x4 c = PERSTEP || i == 0 ? zero4 : ps[j & 1][u];
+                    if constexpr (F16OP) ps[j & 1][u] = w4_mfma(qa[t & 1][i].h, qx[SET][i][u].h, c);
+                    else ps[j & 1][u] = w4_mfma(qa[t & 1][i].b, qx[SET][i][u].b, c);
+                }
+                if (j > 0 && (PERSTEP || i == KS - 1)) flush(j - 1);
+            }
+#pragma unroll
+            for (int it = 0; it < ITEMS; it++)
+                if (it * TM / ITEMS == t) item(it);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        flush(TM * FS - 1);
+        __syncthreads();
+        w4_u32x4* t = b0; b0 = b1; b1 = b2; b2 = t;
+    };
+
+    load(0);
+    store(b0);
+    if (nstages > 1) { load(1); store(b1); }
+    if (nstages > 2) load(2);
+    __syncthreads();
+    int s = 0;
+    const int plain = p.C / (KS * 32) - 3;                // stages s < plain: s + 3 is whole
+    if constexpr (!GRAD && P::X == 1) {
+        if (plain >= 2) {
+            read_qa(b0, 0);
+#pragma unroll
+            for (int t = 0; t < TN; t++) read_qx(0, b0, t);
+            if (p.gsteps % 2)
+                for (; s + 2 <= plain; s += 2) {
+                    body16.template operator()<true, 0>(s);
+                    body16.template operator()<true, 1>(s + 1);
+                }
+            else
+                for (; s + 2 <= plain; s += 2) {
+                    body16.template operator()<false, 0>(s);
+                    body16.template operator()<false, 1>(s + 1);
+                }
+            crem = s * KS % p.gsteps;
+        }
+    } else if (plain >= 2 / KS && (GRAD || p.gsteps % 2 == 0)) {
+        constexpr int D = 2 / KS;
+        read_a(0, b0, 0);
+        read_x(0, b0, 0);
+        if constexpr (GRAD) {
+            for (; s + D <= plain; s += D) body.template operator()<false, false>(s);
+        } else if (p.gsteps == 2) {
+            for (; s + D <= plain; s += D) body.template operator()<true, true>(s);
+        } else {
+            const int gst = p.gsteps / KS;
+            while (s + gst <= plain) {
+                const int e = s + gst - D;
+                body.template operator()<true, false>(s);
+                for (s += D; s < e; s += D) body.template operator()<false, false>(s);
+                body.template operator()<false, true>(s);
+                s += D;
+            }
+        }
+    }
+    for (; s < nstages; s++) {
+        if (s + 2 < nstages) {
+            store(b2);
+            if (s + 3 < nstages) load(s + 3);
+        }
 #pragma unroll
         for (int i = 0; i < KS; i++) {
             if (i > 0 && (s * KS + i) * 32 >= p.C) break;
-            step(buf, i, (s * KS + i + 1) * 32 >= p.C);
+            step(b0, i, (s * KS + i + 1) * 32 >= p.C);
         }
         __syncthreads();
+        w4_u32x4* t = b0; b0 = b1; b1 = b2; b2 = t;
     }
 
     const bool vec = ((uintptr_t)p.y % (4 * sizeof(T)) == 0) && p.ldy % 4 == 0;
@@ -644,22 +839,27 @@ hipError_t w4_launch_bf16(const W4Params&, int scale_type, bool grad, hipStream_
 hipError_t w4_launch_f16(const W4Params&, int scale_type, bool grad, hipStream_t);
 
 #ifdef W4_KERNELS
-template <int DT, int ST, int NT, int GS, bool GRAD>
+template <int DT, int ST, int NT, int MT, int GS, bool GRAD>
 static hipError_t launch_rows(const W4Params& p, hipStream_t st) {
-    constexpr int MT = GRAD ? 2 : 1;
     constexpr int D = DT == GR_DT_F32 || NT > 1 || GRAD ? 1 : 2;
     const int64_t blocks = (int64_t)((p.R + 16 * MT - 1) / (16 * MT)) * ((p.N + 16 * NT - 1) / (16 * NT));
     int waves = blocks >= 2048 ? 4 : blocks >= 512 ? 8 : w4_rows_waves(NT, GRAD);
     if (waves > p.chunks) waves = p.chunks;
-    hipLaunchKernelGGL((k_w4_rows<DT, ST, NT, MT, GS, D, GRAD>), dim3((unsigned)blocks), dim3(waves * 64), (size_t)waves * MT * NT * 1024, st, p);
+    const size_t lds = (size_t)waves * MT * NT * 1024;
+    auto kern = &k_w4_rows<DT, ST, NT, MT, GS, D, GRAD>;
+    if (lds > 64 * 1024) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(waves * 64), lds, st, p);
     return hipGetLastError();
 }
-template <int DT, int ST, int NT, bool GRAD>
+template <int DT, int ST, int NT, int MT, bool GRAD>
 static hipError_t launch_rows(const W4Params& p, hipStream_t st) {
-    if constexpr (GRAD) return launch_rows<DT, ST, NT, 1, true>(p, st);
-    else if (p.gsteps % 4 == 0) return launch_rows<DT, ST, NT, 1, false>(p, st);
-    else if (p.gsteps % 2 == 0) return launch_rows<DT, ST, NT, 2, false>(p, st);
-    else return launch_rows<DT, ST, NT, 4, false>(p, st);
+    if constexpr (GRAD) return launch_rows<DT, ST, NT, MT, 1, true>(p, st);
+    else if (p.gsteps % 4 == 0) return launch_rows<DT, ST, NT, MT, 1, false>(p, st);
+    else if (p.gsteps % 2 == 0) return launch_rows<DT, ST, NT, MT, 2, false>(p, st);
+    else return launch_rows<DT, ST, NT, MT, 4, false>(p, st);
 }
 template <int DT, int ST, bool GRAD, int TM, int TN, int WM, int WN, int KS>
 static hipError_t launch_gemm(const W4Params& p, hipStream_t st) {
@@ -673,10 +873,27 @@ static hipError_t launch_gemm(const W4Params& p, hipStream_t st) {
 }
 template <int DT, int ST, bool GRAD>
 static hipError_t launch_typed(const W4Params& p, hipStream_t st) {
-    if (p.N <= 16) return launch_rows<DT, ST, 1, GRAD>(p, st);
-    if (p.N <= 200) return launch_rows<DT, ST, 2, GRAD>(p, st);
-    if constexpr (GRAD && DT == GR_DT_F32) return launch_gemm<DT, ST, GRAD, 4, 2, 2, 4, 1>(p, st);
-    else if constexpr (DT == GR_DT_F32 || (GRAD && DT == GR_DT_F16)) return launch_gemm<DT, ST, GRAD, 4, 2, 2, 4, 2>(p, st);
+    // Few rows: the smallest tile that leaves at most one workgroup a CU.  A workgroup's time depends on its tile and on the
+    // contraction, hardly on how many there are: 4096 -> 4096 bf16, g = 128, row tiles x batch tiles 1x1 7.5 us, 2x1 9.8, 2x2 14,
+    // 4x2 19, 4x4 30 (gradient 2x1 14, 4x1 20, 4x2 25, 8x2 37).  Many rows: the tiled kernel, whose one round of workgroups
+    // takes 90 us there (f32 110 us; gradient 127 us) and covers 32768 tiles (f32 and f16 gradient 16384).
+    const int64_t tiles = (int64_t)((p.R + 15) / 16) * ((p.N + 15) / 16);        // of 16 x 16 outputs
+    if constexpr (!GRAD) {
+        if (tiles <= 256) return launch_rows<DT, ST, 1, 1, GRAD>(p, st);
+        if (p.N <= 16 || tiles <= 512) return launch_rows<DT, ST, 1, 2, GRAD>(p, st);
+        if (tiles <= 1024) return launch_rows<DT, ST, 2, 2, GRAD>(p, st);
+        if (tiles <= 2048) return launch_rows<DT, ST, 2, 4, GRAD>(p, st);
+        if (tiles <= (DT == GR_DT_F32 ? 6144 : 12288)) return launch_rows<DT, ST, 4, 4, GRAD>(p, st);
+    } else if (p.N <= 16 || tiles <= 12288) {
+        // a workgroup's row tiles share one group: its scales go to the activations
+        const int most = p.gsteps % 4 == 0 ? 8 : p.gsteps % 2 == 0 ? 4 : 2;
+        if (p.N <= 16 || tiles <= 512 || most == 2) return launch_rows<DT, ST, 1, 2, GRAD>(p, st);
+        if (tiles <= 1024) return launch_rows<DT, ST, 1, 4, GRAD>(p, st);
+        if (tiles <= 2048 || most == 4) return launch_rows<DT, ST, 2, 4, GRAD>(p, st);
+        return launch_rows<DT, ST, 2, 8, GRAD>(p, st);
+    }
+    if constexpr (DT == GR_DT_F32 || (GRAD && DT == GR_DT_F16)) return launch_gemm<DT, ST, GRAD, 4, 2, 2, 4, 1>(p, st);
+    else if constexpr (GRAD) return launch_gemm<DT, ST, GRAD, 4, 4, 2, 4, 1>(p, st);
     else return launch_gemm<DT, ST, GRAD, 4, 4, 2, 4, 2>(p, st);
 }
 template <int DT>

@@ -8,7 +8,7 @@ struct gr_w4 {
     gr_ctx* ctx = nullptr;
     int device = 0;
     int M = 0, K = 0, group = 0, G = 0, st = 0, Mp = 0, Kp = 0;
-    bool has_zeros = false;
+    bool has_zeros = false;              // else `zeros` is one row of eights
     char* mem = nullptr;                 // one allocation: pack | transposed pack | scales | zeros | bias
     w4_u32x4 *pack = nullptr, *packT = nullptr;
     void* scales = nullptr;
@@ -47,7 +47,8 @@ __global__ void k_w4_scales(const T* __restrict__ s, int64_t lds, const uint8_t*
     if (id >= (int64_t)G * Mp) return;
     const int m = (int)(id % Mp), g = (int)(id / Mp);
     so[id] = m < M ? s[m * lds + g] : (T)0;
-    if (zo) zo[id] = m < M ? z[m * ldz + g] & 15 : 0;
+    if (z) zo[id] = m < M ? z[m * ldz + g] & 15 : 0;
+    else if (g == 0) zo[id] = 8;
 }
 
 extern "C" void gr_w4_destroy(gr_w4* w) {
@@ -79,7 +80,7 @@ extern "C" int gr_w4_create(gr_ctx* ctx, const uint8_t* q, int64_t ldq, const vo
     w->ctx = ctx; w->device = ctx->device; w->M = M; w->K = K; w->group = group; w->G = G; w->st = scale_type; w->has_zeros = zeros != nullptr;
     w->Mp = (M + 127) / 128 * 128; w->Kp = (K + 127) / 128 * 128;
     const size_t pk = (size_t)w->Mp * w->Kp / 2, ssz = gr_align((size_t)G * w->Mp * dt_size(scale_type));
-    const size_t zsz = zeros ? gr_align((size_t)G * w->Mp) : 0, bsz = bias ? gr_align((size_t)M * 4) : 0;
+    const size_t zsz = gr_align((size_t)(zeros ? G : 1) * w->Mp), bsz = bias ? gr_align((size_t)M * 4) : 0;
     hipError_t e = hipMalloc((void**)&w->mem, pk * (input_grad ? 2 : 1) + ssz + zsz + bsz);
     if (e != hipSuccess) {
         w->mem = nullptr;
@@ -90,7 +91,7 @@ extern "C" int gr_w4_create(gr_ctx* ctx, const uint8_t* q, int64_t ldq, const vo
     w->pack = (w4_u32x4*)m; m += pk;
     if (input_grad) { w->packT = (w4_u32x4*)m; m += pk; }
     w->scales = m; m += ssz;
-    if (zeros) { w->zeros = (uint8_t*)m; m += zsz; }
+    w->zeros = (uint8_t*)m; m += zsz;
     const int64_t nd = (int64_t)(pk / 4), ns = (int64_t)G * w->Mp;
     const dim3 gp((unsigned)((nd + 255) / 256)), gs((unsigned)((ns + 255) / 256));
     if (nd / 256 >= INT_MAX || ns / 256 >= INT_MAX) { gr_w4_destroy(w); return gr_fail(ctx, GR_EINVAL, "gr_w4_create: too many weights"); }
@@ -136,12 +137,13 @@ static int w4_run(gr_ctx* ctx, const gr_w4* w, const char* who, bool grad, const
     if ((int64_t)((p.R + 15) / 16) * ((N + 15) / 16) > INT_MAX) return gr_fail(ctx, GR_EINVAL, "%s: batch too large", who);
     p.pack = grad ? w->packT : w->pack;
     p.scales = w->scales; p.zeros = w->zeros; p.Mp = w->Mp;
+    p.zstride = w->has_zeros ? w->Mp : 0;
     p.chunks = (grad ? w->Mp : w->Kp) / W4_CHUNK;
     p.gsteps = w->group / 32;
     p.x = x; p.y = y; p.bias = w->bias; p.gate = gate;
     p.N = N; p.ldx = ldx; p.ldy = ldy; p.ldg = ldg; p.relu = relu;
     const double fl = 2.0 * (double)N * w->M * w->K;
-    const double by = (double)w->M * w->K / 2 + (double)w->M * w->G * (dt_size(w->st) + (w->zeros ? 1 : 0)) + (double)N * (w->M + w->K) * es;
+    const double by = (double)w->M * w->K / 2 + (double)w->M * w->G * (dt_size(w->st) + (w->has_zeros ? 1 : 0)) + (double)N * (w->M + w->K) * es;
     ProfScope ps(ctx, grad ? "k_w4_grad" : "k_w4_forward", st, fl, by);
     const hipError_t e = w4_launch(p, dt, w->st, grad, st);
     GR_HIP(ctx, e);
