@@ -61,6 +61,8 @@ SIGNATURES = {
     "gr_pg_local_logits": (_i, [_vp, _vp, _vp, _i, _vp, _vp]),
     "gr_pg_masking_defense": (_i, [_vp, _vp, _i, _i, _i, _i, _i, _f, _vp, _vp, _vp]),
     "gr_model_input_grad": (_i, [_vp, _vp, _vp, _i, _i, _vp, _vp, _vp]),
+    "gr_model_input_grad_topk": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _i, _i64, _vp, _f, _vp, _vp, _vp, _vp]),
+    "gr_model_set_linear_w4": (_i, [_vp, _i, _vp]),
     "gr_tr_hits": (_i, [_vp, _vp, _vp, _i, _i, _vp, _vp, _i, _i, _i, _vp, _f, _i, _i, _i64, _i64, _vp, _vp, _vp, _vp]),
     "gr_w4_create": (_i, [_vp, _vp, _i64, _vp, _i, _i64, _vp, _i64, _vp, _i, _i, _i, _i, _vp, C.POINTER(_vp)]),
     "gr_w4_destroy": (None, [_vp]),
@@ -211,6 +213,11 @@ def to_dev(a):
     elif a.is_cuda and a.dtype == torch.float32 and a.is_contiguous() and a.device.index == torch.cuda.current_device():
         return a                                    # already in place: the evaluator's calls pass through here twice
     return a.to(device=f"cuda:{device_index()}", dtype=torch.float32).contiguous()
+
+
+def to_index(a, device):
+    """int64 contiguous tensor on `device`."""
+    return torch.as_tensor(a).to(device=device, dtype=torch.int64).contiguous()
 
 
 def _p(t):
@@ -392,6 +399,7 @@ class Model:
         ptrs = (_vp * len(keep))(*[t.ctypes.data for t in keep])
         numel = (C.c_int64 * len(keep))(*[t.size for t in keep])
         self._h = _vp()
+        self._w4 = {}
         self.kind = kind
         if kind == "gtsrb":
             rc = lib.gr_model_load_gtsrb(self._ctx, ptrs, numel, len(keep), C.byref(self._h))
@@ -439,6 +447,36 @@ class Model:
         _check(self._ctx, load_library().gr_model_input_grad(self._ctx, self._h, _p(xd), n, int(target), _p(logits), _p(gx),
                                                              _stream()), "gr_model_input_grad")
         return logits, gx
+
+    def input_grad_topk(self, x, teacher):
+        """input_grad for a soft target: (logits [N,ncls], d loss_n / d x_n, loss [N]) as CUDA tensors, loss_n = the
+        distillation loss of logits_n against `teacher` (distill.TeacherTop of one row, or of N rows)."""
+        xd = to_dev(x)
+        if xd.dim() == 3:
+            xd = xd[None]
+        n = xd.shape[0]
+        index, value = to_index(teacher.index, xd.device), to_dev(teacher.value)
+        if index.dim() == 1:
+            index, value = index[None], value[None]
+        lse = None if teacher.lse is None else to_dev(teacher.lse).reshape(-1)
+        rows = index.shape[0]
+        if index.shape != value.shape or rows not in (1, n) or (lse is not None and lse.numel() != rows):
+            raise GraphiteHipError(f"teacher of shape {tuple(index.shape)} / {tuple(value.shape)} for {n} images: one row, or one per image")
+        k = index.shape[1]
+        logits = torch.empty((n, self.num_classes), device=xd.device, dtype=torch.float32)
+        loss = torch.empty((n,), device=xd.device, dtype=torch.float32)
+        gx = torch.empty_like(xd)
+        _check(self._ctx, load_library().gr_model_input_grad_topk(
+            self._ctx, self._h, _p(xd), n, _p(index), _p(value), k, 0 if rows == 1 else k, _p(lse), float(teacher.tau), _p(loss),
+            _p(logits), _p(gx), _stream()), "gr_model_input_grad_topk")
+        return logits, gx, loss
+
+    def set_linear_w4(self, layer, w4):
+        """Linear layer number `layer` (GTSRBNet 0 = fc5_1, 1 = fc6_1, 2 = fc7_1; the others 0 = fc) on 4-bit weights
+        (linear_w4.LinearW4), None: the float layer again."""
+        _check(self._ctx, load_library().gr_model_set_linear_w4(self._h, int(layer), None if w4 is None else w4._h),
+               "gr_model_set_linear_w4")
+        self._w4[int(layer)] = w4                        # the model uses the layer's memory
 
     def forward(self, x):
         """x: [N,3,32,32] (any device) -> logits CUDA tensor [N,ncls]."""

@@ -506,11 +506,10 @@ extern "C" int gr_pg_local_logits(gr_ctx* ctx, gr_model* m, const float* x, int 
     return GR_OK;
 }
 
-extern "C" int gr_model_input_grad(gr_ctx* ctx, gr_model* m, const float* x, int N, int target, float* logits,
-                                   float* grad_x, void* stream) {
-    NEED_CTX();
-    if (!m || !x || !grad_x || N < 0) return gr_fail(ctx, GR_EINVAL, "gr_model_input_grad: bad arguments");
-    if (net_pg_out_size(m) > 0) return gr_fail(ctx, GR_EINVAL, "gr_model_input_grad: the PatchGuard classifier has no gradient path (the reference has none either)");
+static int model_input_grad(gr_ctx* ctx, gr_model* m, const char* who, const float* x, int N, int target, const NetSoftTarget* soft,
+                            float* logits, float* grad_x, void* stream) {
+    if (!m || !x || !grad_x || N < 0) return gr_fail(ctx, GR_EINVAL, "%s: bad arguments", who);
+    if (net_pg_out_size(m) > 0) return gr_fail(ctx, GR_EINVAL, "%s: the PatchGuard classifier has no gradient path (the reference has none either)", who);
     hipStream_t st = (hipStream_t)stream;
     const int ncls = gr_model_num_classes(m);
     // the pass keeps every activation: ~0.8 MB per image for GTSRBNet, ~17 MB for WideResNet-34-10
@@ -523,10 +522,31 @@ extern "C" int gr_model_input_grad(gr_ctx* ctx, gr_model* m, const float* x, int
     if (rc) return rc;
     for (int n0 = 0; n0 < N; n0 += chunk) {
         int nb = N - n0 < chunk ? N - n0 : chunk;
-        if ((rc = net_input_grad(ctx, m, x + (size_t)n0 * 3072, nb, target, logits ? logits + (size_t)n0 * ncls : nullptr,
+        NetSoftTarget part;
+        if (soft) {
+            part = *soft;
+            part.index += n0 * part.ld_top;
+            part.value += n0 * part.ld_top;
+            if (part.lse && part.ld_top) part.lse += n0;
+            if (part.loss) part.loss += n0;
+        }
+        if ((rc = net_input_grad(ctx, m, x + (size_t)n0 * 3072, nb, target, soft ? &part : nullptr, logits ? logits + (size_t)n0 * ncls : nullptr,
                                  grad_x + (size_t)n0 * 3072, ctx->ws, ctx->ws_bytes, st))) return rc;
     }
     return GR_OK;
+}
+extern "C" int gr_model_input_grad(gr_ctx* ctx, gr_model* m, const float* x, int N, int target, float* logits,
+                                   float* grad_x, void* stream) {
+    NEED_CTX();
+    return model_input_grad(ctx, m, "gr_model_input_grad", x, N, target, nullptr, logits, grad_x, stream);
+}
+extern "C" int gr_model_input_grad_topk(gr_ctx* ctx, gr_model* m, const float* x, int N, const int64_t* index, const float* value, int k,
+                                        int64_t ld_top, const float* teacher_lse, float tau, float* loss, float* logits, float* grad_x,
+                                        void* stream) {
+    NEED_CTX();
+    if (!index || !value || k < 1 || (ld_top != 0 && ld_top < k)) return gr_fail(ctx, GR_EINVAL, "gr_model_input_grad_topk: bad arguments");
+    const NetSoftTarget soft = {index, value, teacher_lse, k, ld_top, tau, loss};
+    return model_input_grad(ctx, m, "gr_model_input_grad_topk", x, N, 0, &soft, logits, grad_x, stream);
 }
 
 // ---------------------------------------------------------------------------------------------

@@ -130,7 +130,14 @@ int net_tie_last(const gr_model*);
 // PatchGuard models: local logits [N,h,h,ncls] of N [3,32,32] inputs (x_chw == nullptr: NHWC4 input in place)
 int net_pg_local(gr_ctx*, gr_model*, const float* x_chw, int N, float* local, char* ws, size_t ws_bytes, hipStream_t);
 int net_pg_out_size(const gr_model*);
-// d CE(logits_n, target) / d x_n (GTSRBNet): forward with every activation kept, then the transposed layers
-int net_input_grad(gr_ctx*, gr_model*, const float* x_chw, int N, int target, float* logits_or_null, float* grad_x, char* ws,
-                   size_t ws_bytes, hipStream_t);
+// d loss / d x_n: forward with every activation kept, then the transposed layers.  loss = CE(logits_n, target), or the
+// distillation loss of `soft` (gr_distill_topk) when that is given
+struct NetSoftTarget { const int64_t* index; const float* value; const float* lse; int k; int64_t ld_top; float tau; float* loss; };
+int net_input_grad(gr_ctx*, gr_model*, const float* x_chw, int N, int target, const NetSoftTarget* soft, float* logits_or_null,
+                   float* grad_x, char* ws, size_t ws_bytes, hipStream_t);
+
+// ---- w4.hip ----
+gr_ctx* w4_ctx(const gr_w4*);
+int w4_out_features(const gr_w4*);
+int w4_in_features(const gr_w4*);
 size_t net_grad_workspace_bytes(const gr_model*, int N);

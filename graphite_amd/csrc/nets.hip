@@ -52,6 +52,7 @@ struct gr_model {
                              // bit 7: keep the activations between them f32 in HBM (they are bf16 when all 7 layers are)
     int ncls = 0;
     std::vector<void*> allocs;
+    const gr_w4* w4[3] = {nullptr, nullptr, nullptr};   // 4-bit linear layers (gr_model_set_linear_w4): GTSRBNet fc5, fc6, fc7; the others' only one
     // GTSRBNet
     float* c11 = nullptr;    // conv1_1: 9 weights + 3 biases
     Layer g[9];              // conv2_1 .. fc7_1
@@ -487,7 +488,26 @@ extern "C" int gr_model_set_precision(gr_model* m, int precision) {
         if (!any) return gr_fail(m->ctx, GR_EINVAL, "gr_model_set_precision: this WideResNet has no layer the bf16 kernels cover "
                                                      "(stride-1 3x3 convs with Cout %% 160 == 0)");
     }
+    if (precision == GR_PREC_BF16 && m->kind == 1 && (m->w4[0] || m->w4[1] || m->w4[2]))
+        return gr_fail(m->ctx, GR_EINVAL, "gr_model_set_precision: this model has 4-bit linear layers (gr_model_set_linear_w4), which run in float32");
     m->precision = precision;
+    return GR_OK;
+}
+extern "C" int gr_model_set_linear_w4(gr_model* m, int layer, const gr_w4* w) {
+    if (!m) return GR_EINVAL;
+    const int n = m->kind == 1 ? 3 : 1;
+    if (layer < 0 || layer >= n) return gr_fail(m->ctx, GR_EINVAL, "gr_model_set_linear_w4: no linear layer %d", layer);
+    if (w) {
+        static const int gm[3] = {1024, 1024, 43}, gk[3] = {2048, 1024, 1024};
+        const int M = m->kind == 1 ? gm[layer] : m->ncls;
+        const int K = m->kind == 1 ? gk[layer] : m->kind == 2 ? m->ch[3] : m->bag_fc.CinT;
+        if (w4_ctx(w) != m->ctx) return gr_fail(m->ctx, GR_ESTATE, "gr_model_set_linear_w4: the layer belongs to another context");
+        if (w4_out_features(w) != M || w4_in_features(w) != K)
+            return gr_fail(m->ctx, GR_EINVAL, "gr_model_set_linear_w4: layer %d is %d -> %d, given %d -> %d", layer, K, M, w4_in_features(w), w4_out_features(w));
+        if (m->kind == 1 && m->precision == GR_PREC_BF16)
+            return gr_fail(m->ctx, GR_EINVAL, "gr_model_set_linear_w4: 4-bit linear layers run in float32; set GR_PREC_F32 first");
+    }
+    m->w4[layer] = w;
     return GR_OK;
 }
 extern "C" int gr_model_get_precision(const gr_model* m) { return m ? m->precision : GR_EINVAL; }
@@ -991,6 +1011,38 @@ static bool use_igemm_convs() {      // GRAPHITE_CONV=igemm selects the im2col-c
     return v == 1;
 }
 
+// fc5's activations between the NHWC order of the conv kernels (k = s*128 + c) and the layer's own NCHW order (k = c*16 + s,
+// GTSRBNet.py:47): the groups of its 4-bit weights run along the latter.  TO_CHW: NHWC -> NCHW.
+template <bool TO_CHW>
+__global__ void k_fc5_order(const float* __restrict__ in, int64_t n, float* __restrict__ out) {
+    const int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (id >= n) return;
+    const int k = (int)(id & 2047), c = k >> 4, s = k & 15;
+    const int64_t chw = id, nhwc = (id - k) + s * 128 + c;
+    if (TO_CHW) out[chw] = in[nhwc];
+    else out[nhwc] = in[chw];
+}
+static int fc5_order(gr_ctx* ctx, const float* in, int N, float* out, bool to_chw, hipStream_t st) {
+    const int64_t n = (int64_t)N * 2048;
+    const dim3 grid((unsigned)((n + 255) / 256));
+    if (to_chw) hipLaunchKernelGGL(k_fc5_order<true>, grid, dim3(256), 0, st, in, n, out);
+    else hipLaunchKernelGGL(k_fc5_order<false>, grid, dim3(256), 0, st, in, n, out);
+    GR_HIP(ctx, hipGetLastError());
+    return GR_OK;
+}
+// GTSRBNet's linear layer l (0 = fc5, 1 = fc6, 2 = fc7) of N rows; tmp: N * 2048 floats, used by a 4-bit fc5
+static int gtsrb_fc(gr_ctx* ctx, gr_model* m, int l, const float* in, int N, float* out, float* tmp, hipStream_t st) {
+    const Layer& L = m->g[6 + l];
+    if (!m->w4[l]) return run_conv(ctx, L, in, N, 1, 1, nullptr, nullptr, out, nullptr, l < 2, false, st);
+    if (l == 0) {
+        const int rc = fc5_order(ctx, in, N, tmp, true, st);
+        if (rc) return rc;
+        in = tmp;
+    }
+    const int64_t K = l == 0 ? 2048 : 1024, M = l == 2 ? 43 : 1024;
+    return gr_linear_w4(ctx, m->w4[l], in, GR_DT_F32, N, K, l < 2, out, M, st);
+}
+
 static int gtsrb_forward(gr_ctx* ctx, gr_model* m, const float* x, int N, float* logits, float* ws, hipStream_t st) {
     float* x4 = ws;
     float* A = x4 + (size_t)N * 4096;
@@ -1045,9 +1097,9 @@ static int gtsrb_forward(gr_ctx* ctx, gr_model* m, const float* x, int N, float*
         if ((rc = run_gtsrb_halo(ctx, m->g[3], 3, A, N, 16, Bf, st))) return rc;
         if ((rc = run_gtsrb_halo(ctx, m->g[4], 4, Bf, N, 8, A, st))) return rc;
         if ((rc = run_gtsrb_halo(ctx, m->g[5], 5, A, N, 8, Bf, st))) return rc;
-        if ((rc = run_conv(ctx, m->g[6], Bf, N, 1, 1, nullptr, nullptr, A, nullptr, true, false, st))) return rc;     // fc5
-        if ((rc = run_conv(ctx, m->g[7], A, N, 1, 1, nullptr, nullptr, Bf, nullptr, true, false, st))) return rc;     // fc6
-        return run_conv(ctx, m->g[8], Bf, N, 1, 1, nullptr, nullptr, logits, nullptr, false, false, st);             // fc7
+        if ((rc = gtsrb_fc(ctx, m, 0, Bf, N, A, A + (size_t)N * 8192, st))) return rc;
+        if ((rc = gtsrb_fc(ctx, m, 1, A, N, Bf, nullptr, st))) return rc;
+        return gtsrb_fc(ctx, m, 2, Bf, N, logits, nullptr, st);
     }
     if ((rc = run_conv(ctx, m->g[0], x4, N, 32, 32, nullptr, nullptr, A, nullptr, true, false, st))) return rc;   // conv2_1
     if ((rc = run_conv(ctx, m->g[1], A, N, 32, 32, nullptr, nullptr, Bf, nullptr, true, true, st))) return rc;    // conv2_2+pool
@@ -1055,9 +1107,9 @@ static int gtsrb_forward(gr_ctx* ctx, gr_model* m, const float* x, int N, float*
     if ((rc = run_conv(ctx, m->g[3], A, N, 16, 16, nullptr, nullptr, Bf, nullptr, true, true, st))) return rc;    // conv3_2+pool
     if ((rc = run_conv(ctx, m->g[4], Bf, N, 8, 8, nullptr, nullptr, A, nullptr, true, false, st))) return rc;     // conv4_1
     if ((rc = run_conv(ctx, m->g[5], A, N, 8, 8, nullptr, nullptr, Bf, nullptr, true, true, st))) return rc;      // conv4_2+pool
-    if ((rc = run_conv(ctx, m->g[6], Bf, N, 1, 1, nullptr, nullptr, A, nullptr, true, false, st))) return rc;     // fc5
-    if ((rc = run_conv(ctx, m->g[7], A, N, 1, 1, nullptr, nullptr, Bf, nullptr, true, false, st))) return rc;     // fc6
-    return run_conv(ctx, m->g[8], Bf, N, 1, 1, nullptr, nullptr, logits, nullptr, false, false, st);             // fc7
+    if ((rc = gtsrb_fc(ctx, m, 0, Bf, N, A, A + (size_t)N * 8192, st))) return rc;
+    if ((rc = gtsrb_fc(ctx, m, 1, A, N, Bf, nullptr, st))) return rc;
+    return gtsrb_fc(ctx, m, 2, Bf, N, logits, nullptr, st);
 }
 
 static int wrn_forward(gr_ctx* ctx, gr_model* m, const float* x, int N, float* logits, float* ws, hipStream_t st) {
@@ -1109,6 +1161,7 @@ static int wrn_forward(gr_ctx* ctx, gr_model* m, const float* x, int N, float* l
     int C = m->ch[3];
     hipLaunchKernelGGL(k_avgpool, dim3((N * C + 255) / 256), dim3(256), 0, st, o, N, H * H, C, u);
     GR_HIP(ctx, hipGetLastError());
+    if (m->w4[0]) return gr_linear_w4(ctx, m->w4[0], u, GR_DT_F32, N, m->ch[3], 0, logits, m->ncls, st);
     return run_conv(ctx, m->wfc, u, N, 1, 1, nullptr, nullptr, logits, nullptr, false, false, st);
 }
 
@@ -1179,25 +1232,42 @@ __global__ void k_input_grad(const float* __restrict__ g3, const float4* __restr
     for (int i = 0; i < 3; i++) o[i * 1024] = r0 * c11[0 * 3 + i] + r1 * c11[1 * 3 + i] + r2 * c11[2 * 3 + i];
 }
 
+// d loss / d logits into a 64-wide row (zero padded): cross entropy to `target`, or the distillation loss of `soft`
+__global__ void k_zero(float* __restrict__ p, int64_t n) {
+    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i < n) p[i] = 0.f;
+}
+static int logit_grad(gr_ctx* ctx, const gr_model* m, const float* logits, int N, int target, const NetSoftTarget* soft, float* g64,
+                      hipStream_t st) {
+    if (!soft) {
+        hipLaunchKernelGGL(k_ce_grad, dim3((N + 255) / 256), dim3(256), 0, st, logits, N, m->ncls, target, g64);
+        GR_HIP(ctx, hipGetLastError());
+        return GR_OK;
+    }
+    hipLaunchKernelGGL(k_zero, dim3((unsigned)(((int64_t)N * 64 + 255) / 256)), dim3(256), 0, st, g64, (int64_t)N * 64);
+    return gr_distill_topk(ctx, logits, GR_DT_F32, N, m->ncls, m->ncls, soft->index, soft->value, GR_DT_F32, soft->k, soft->ld_top,
+                           soft->lse, soft->tau, nullptr, soft->loss, g64, 64, st);
+}
+
 static size_t grad_floats_per_image() {
     //     x4     a21     a22     p2     a31     a32     p3     a41    a42    p4     f5     f6    lg   g64   gA      gB
     return 4096 + 32768 + 32768 + 8192 + 16384 + 16384 + 4096 + 8192 + 8192 + 2048 + 1024 + 1024 + 64 + 64 + 32768 + 32768;
 }
 static size_t wrn_grad_floats_per_image(const gr_model* m);
-static int wrn_input_grad(gr_ctx* ctx, gr_model* m, const float* x, int N, int target, float* logits_out, float* gx,
-                          float* w, hipStream_t st);
+static int wrn_input_grad(gr_ctx* ctx, gr_model* m, const float* x, int N, int target, const NetSoftTarget* soft, float* logits_out,
+                          float* gx, float* w, hipStream_t st);
 size_t net_grad_workspace_bytes(const gr_model* m, int N) {
     const size_t per = m->kind == 2 ? wrn_grad_floats_per_image(m) : grad_floats_per_image();
     return gr_align(per * sizeof(float) * (size_t)N);
 }
 
 // logits (optional) and d CE(logits_n, target) / d x_n for N images; GTSRBNet only.
-int net_input_grad(gr_ctx* ctx, gr_model* m, const float* x, int N, int target, float* logits_out, float* gx, char* wsb,
-                   size_t ws_bytes, hipStream_t st) {
+int net_input_grad(gr_ctx* ctx, gr_model* m, const float* x, int N, int target, const NetSoftTarget* soft, float* logits_out, float* gx,
+                   char* wsb, size_t ws_bytes, hipStream_t st) {
     if (N <= 0) return GR_OK;
-    if (target < 0 || target >= m->ncls) return gr_fail(ctx, GR_EINVAL, "target %d out of range", target);
+    if (!soft && (target < 0 || target >= m->ncls)) return gr_fail(ctx, GR_EINVAL, "target %d out of range", target);
     if (ws_bytes < net_grad_workspace_bytes(m, N)) return gr_fail(ctx, GR_ESTATE, "net_input_grad: workspace too small");
-    if (m->kind == 2) return wrn_input_grad(ctx, m, x, N, target, logits_out, gx, (float*)wsb, st);
+    if (m->kind == 2) return wrn_input_grad(ctx, m, x, N, target, soft, logits_out, gx, (float*)wsb, st);
     if (m->kind != 1) return gr_fail(ctx, GR_EINVAL, "unknown model kind");
     float* w = (float*)wsb;
     auto take = [&](size_t per) { float* p = w; w += per * (size_t)N; return p; };
@@ -1217,15 +1287,21 @@ int net_input_grad(gr_ctx* ctx, gr_model* m, const float* x, int N, int target, 
     if ((rc = run_conv(ctx, m->g[4], p3, N, 8, 8, nullptr, nullptr, a41, nullptr, true, false, st))) return rc;
     if ((rc = run_conv(ctx, m->g[5], a41, N, 8, 8, nullptr, nullptr, a42, nullptr, true, false, st))) return rc;
     hipLaunchKernelGGL(k_maxpool2_fwd, blocks((size_t)N * 2048), dim3(256), 0, st, a42, N, 8, 8, 128, p4);
-    if ((rc = run_conv(ctx, m->g[6], p4, N, 1, 1, nullptr, nullptr, f5, nullptr, true, false, st))) return rc;
-    if ((rc = run_conv(ctx, m->g[7], f5, N, 1, 1, nullptr, nullptr, f6, nullptr, true, false, st))) return rc;
+    if ((rc = gtsrb_fc(ctx, m, 0, p4, N, f5, gA, st))) return rc;
+    if ((rc = gtsrb_fc(ctx, m, 1, f5, N, f6, nullptr, st))) return rc;
     float* lgp = logits_out ? logits_out : lg;
-    if ((rc = run_conv(ctx, m->g[8], f6, N, 1, 1, nullptr, nullptr, lgp, nullptr, false, false, st))) return rc;
+    if ((rc = gtsrb_fc(ctx, m, 2, f6, N, lgp, nullptr, st))) return rc;
     // ---- backward: every transposed layer gates its output with the ReLU of the activation it produces the gradient of ----
-    hipLaunchKernelGGL(k_ce_grad, blocks((size_t)N), dim3(256), 0, st, lgp, N, m->ncls, target, g64);
-    if ((rc = run_conv(ctx, m->gb[8], g64, N, 1, 1, nullptr, nullptr, gA, nullptr, false, false, st, f6))) return rc;   // d f6
-    if ((rc = run_conv(ctx, m->gb[7], gA, N, 1, 1, nullptr, nullptr, gB, nullptr, false, false, st, f5))) return rc;    // d f5
-    if ((rc = run_conv(ctx, m->gb[6], gB, N, 1, 1, nullptr, nullptr, gA, nullptr, false, false, st))) return rc;        // d p4
+    if ((rc = logit_grad(ctx, m, lgp, N, target, soft, g64, st))) return rc;
+    if (m->w4[2]) { if ((rc = gr_linear_w4_input_grad(ctx, m->w4[2], g64, GR_DT_F32, N, 64, f6, 1024, gA, 1024, st))) return rc; }   // d f6
+    else if ((rc = run_conv(ctx, m->gb[8], g64, N, 1, 1, nullptr, nullptr, gA, nullptr, false, false, st, f6))) return rc;
+    if (m->w4[1]) { if ((rc = gr_linear_w4_input_grad(ctx, m->w4[1], gA, GR_DT_F32, N, 1024, f5, 1024, gB, 1024, st))) return rc; }  // d f5
+    else if ((rc = run_conv(ctx, m->gb[7], gA, N, 1, 1, nullptr, nullptr, gB, nullptr, false, false, st, f5))) return rc;
+    if (m->w4[0]) {                                                                                                                 // d p4
+        float* chw = gB + (size_t)N * 1024;
+        if ((rc = gr_linear_w4_input_grad(ctx, m->w4[0], gB, GR_DT_F32, N, 1024, nullptr, 0, chw, 2048, st))) return rc;
+        if ((rc = fc5_order(ctx, chw, N, gA, false, st))) return rc;
+    } else if ((rc = run_conv(ctx, m->gb[6], gB, N, 1, 1, nullptr, nullptr, gA, nullptr, false, false, st))) return rc;
     hipLaunchKernelGGL(k_maxpool2_relu_bwd, blocks((size_t)N * 2048), dim3(256), 0, st, a42, gA, N, 8, 8, 128, gB);      // d a42
     if ((rc = run_conv(ctx, m->gb[5], gB, N, 8, 8, nullptr, nullptr, gA, nullptr, false, false, st, a41))) return rc;    // d a41
     if ((rc = run_conv(ctx, m->gb[4], gA, N, 8, 8, nullptr, nullptr, gB, nullptr, false, false, st))) return rc;         // d p3
@@ -1311,8 +1387,8 @@ static size_t wrn_grad_floats_per_image(const gr_model* m) {
     return 4096 + 3 * wrn_big(m) + keep + m->ch[3] + 64 + 64 + 5 * wrn_gbig(m);
 }
 
-static int wrn_input_grad(gr_ctx* ctx, gr_model* m, const float* x, int N, int target, float* logits_out, float* gx,
-                          float* w, hipStream_t st) {
+static int wrn_input_grad(gr_ctx* ctx, gr_model* m, const float* x, int N, int target, const NetSoftTarget* soft, float* logits_out,
+                          float* gx, float* w, hipStream_t st) {
     const size_t big = wrn_big(m);
     auto take = [&](size_t per) { float* p = w; w += per * (size_t)N; return p; };
     auto blocks = [](size_t n) { return dim3((unsigned)((n + 255) / 256)); };
@@ -1360,10 +1436,12 @@ static int wrn_input_grad(gr_ctx* ctx, gr_model* m, const float* x, int N, int t
     const int C3 = m->ch[3], P = H * H;
     hipLaunchKernelGGL(k_avgpool, blocks((size_t)N * C3), dim3(256), 0, st, OF, N, P, C3, pooled);
     float* lgp = logits_out ? logits_out : lg;
-    if ((rc = run_conv(ctx, m->wfc, pooled, N, 1, 1, nullptr, nullptr, lgp, nullptr, false, false, st))) return rc;
+    if (m->w4[0]) { if ((rc = gr_linear_w4(ctx, m->w4[0], pooled, GR_DT_F32, N, C3, 0, lgp, m->ncls, st))) return rc; }
+    else if ((rc = run_conv(ctx, m->wfc, pooled, N, 1, 1, nullptr, nullptr, lgp, nullptr, false, false, st))) return rc;
     // ---- backward ----
-    hipLaunchKernelGGL(k_ce_grad, blocks((size_t)N), dim3(256), 0, st, lgp, N, m->ncls, target, g64);
-    if ((rc = run_conv(ctx, m->wfcT, g64, N, 1, 1, nullptr, nullptr, gA, nullptr, false, false, st))) return rc;       // d pooled
+    if ((rc = logit_grad(ctx, m, lgp, N, target, soft, g64, st))) return rc;
+    if (m->w4[0]) { if ((rc = gr_linear_w4_input_grad(ctx, m->w4[0], g64, GR_DT_F32, N, 64, nullptr, 0, gA, C3, st))) return rc; }     // d pooled
+    else if ((rc = run_conv(ctx, m->wfcT, g64, N, 1, 1, nullptr, nullptr, gA, nullptr, false, false, st))) return rc;
     hipLaunchKernelGGL(k_pool_bn_relu_bwd, blocks((size_t)N * P * C3), dim3(256), 0, st, gA, OF, m->bnf.scale, N, P, C3, gY);
     for (size_t bi = nb; bi-- > 0;) {
         WrnBlock& b = m->blocks[bi];
@@ -1456,6 +1534,7 @@ int net_pg_local(gr_ctx* ctx, gr_model* m, const float* x, int N, float* local, 
         float* tmp = X; X = T1; T1 = tmp;
         H = Ho;
     }
+    if (m->w4[0]) return gr_linear_w4(ctx, m->w4[0], X, GR_DT_F32, (int64_t)N * H * H, m->bag_fc.CinT, 0, local, m->ncls, st);
     return run_conv(ctx, m->bag_fc, X, N, H, H, nullptr, nullptr, local, nullptr, false, false, st);
 }
 

@@ -51,6 +51,10 @@ __global__ void k_w4_scales(const T* __restrict__ s, int64_t lds, const uint8_t*
     else if (g == 0) zo[id] = 8;
 }
 
+gr_ctx* w4_ctx(const gr_w4* w) { return w->ctx; }
+int w4_out_features(const gr_w4* w) { return w->M; }
+int w4_in_features(const gr_w4* w) { return w->K; }
+
 extern "C" void gr_w4_destroy(gr_w4* w) {
     if (!w) return;
     if (w->mem) {

@@ -118,11 +118,15 @@ def tr_error_rates(model, image, masks, thetas, transforms, target, **kw):
     return [(1.0 - int(h) * 1.0 / T, T) for h in hits]
 
 
-def eot_gradient(model, image, adv, mask, transforms, target, pt_file='inputs/GTSRB/Points/14.csv', normalize=True):
+def eot_gradient(model, image, adv, mask, transforms, target, pt_file='inputs/GTSRB/Points/14.csv', normalize=True,
+                 teacher=None):
     """One step of the whitebox EOT loop (reference whitebox/whitebox_attack.py:149-162), everything on the GPU:
     x_t = transform_wb(image, adv, mask, transform_t) [- 0.5]; loss_t = CrossEntropy(model(x_t), target);
     returns (mean over t of d loss_t / d adv  [3,H,W] CUDA, logits [T,ncls] CUDA).
-    Three launches groups: gr_wb_forward, gr_model_input_grad, gr_wb_backward."""
+    Three launches groups: gr_wb_forward, gr_model_input_grad, gr_wb_backward.
+    teacher: a distill.TeacherTop (one row, or one per transform) -- loss_t is then the distillation loss of model(x_t)
+    against the teacher's top classes, e.g. the few scores a victim answers with for the target image, and `target` is not
+    used (gr_model_input_grad_topk)."""
     import torch
     from . import transforms as T
     hip_model = getattr(model, "hip_model", model)
@@ -134,6 +138,9 @@ def eot_gradient(model, image, adv, mask, transforms, target, pt_file='inputs/GT
     x = _hip.wb_forward(o, a, m, tab)
     if normalize:
         x = x - 0.5
-    logits, gx = hip_model.input_grad(x, target)
+    if teacher is None:
+        logits, gx = hip_model.input_grad(x, target)
+    else:
+        logits, gx, _ = hip_model.input_grad_topk(x, teacher)
     g = _hip.wb_backward(o, a, m, tab, gx)
     return g / float(len(tab)), logits

@@ -122,21 +122,23 @@ def attack_network(model, img_v, img_t, mask, lbl_v, lbl_t, pt_file, scorefile, 
     return res
 
 
-def _load_weights(model, checkpoint, key, synth_fn):
+def _load_weights(model, checkpoint, key, synth_fn, linear_w4=0):
+    """linear_w4 > 0: the victim's linear layers on 4-bit weights with a scale per that many inputs."""
     if checkpoint:
         sd = torch.load(checkpoint, map_location="cpu", weights_only=True)
-        model.load_state_dict(sd[key] if key and key in sd else sd)
+        sd = sd[key] if key and key in sd else sd
     else:
         print("no --checkpoint given: using graphite_amd.synth seeded weights")
-        model.load_state_dict(synth_fn())
-    return model
+        sd = synth_fn()
+    model.load_state_dict(sd)
+    return model.quantize_linear(sd, linear_w4) if linear_w4 else model
 
 
 def attack_GTSRB(img_v, img_t, mask, lbl_v, lbl_t, pt_file, scorefile, heatmap, coarseerror, reduceerror, beta=1,
                  num_xforms_mask=100, num_xforms_boost=1000, net_size=32, noise_size=32, joint_iters=1, checkpoint=None,
-                 **kw):
+                 linear_w4=0, **kw):
     from . import synth
-    model = _load_weights(GTSRBNet(), checkpoint, 'model_state_dict', synth.gtsrb_state_dict)
+    model = _load_weights(GTSRBNet(), checkpoint, 'model_state_dict', synth.gtsrb_state_dict, linear_w4)
     return attack_network(model, img_v, img_t, mask, lbl_v, lbl_t, pt_file, scorefile, heatmap, coarseerror, reduceerror,
                           beta, num_xforms_mask, num_xforms_boost, net_size, noise_size, model_type='GTSRB',
                           joint_iters=joint_iters, **kw)
@@ -144,9 +146,9 @@ def attack_GTSRB(img_v, img_t, mask, lbl_v, lbl_t, pt_file, scorefile, heatmap, 
 
 def attack_CIFAR(img_v, img_t, mask, lbl_v, lbl_t, pt_file, scorefile, heatmap, coarseerror, reduceerror, beta=1,
                  num_xforms_mask=100, num_xforms_boost=1000, net_size=32, noise_size=32, joint_iters=1, image_id='',
-                 checkpoint=None, **kw):
+                 checkpoint=None, linear_w4=0, **kw):
     from . import synth
-    model = _load_weights(WideResNet(num_classes=10), checkpoint, None, synth.wrn_state_dict)
+    model = _load_weights(WideResNet(num_classes=10), checkpoint, None, synth.wrn_state_dict, linear_w4)
     return attack_network(model, img_v, img_t, mask, lbl_v, lbl_t, pt_file, scorefile, heatmap, coarseerror, reduceerror,
                           beta, num_xforms_mask, num_xforms_boost, net_size, noise_size, model_type='CIFAR',
                           joint_iters=joint_iters, image_id=image_id, **kw)
@@ -157,6 +159,8 @@ def main(argv=None):
     extra = argparse.ArgumentParser(add_help=False)
     extra.add_argument('--checkpoint')
     extra.add_argument('--no_outputs', action='store_true')
+    extra.add_argument('--linear_w4', type=int, default=0, metavar='GROUP',
+                       help="attack the victim as a 4-bit deployment runs it: linear layers on 4-bit weights, one scale per GROUP inputs")
     ex, rest = extra.parse_known_args(argv)
     args = parsearguments.getarguments(rest)
     torch.manual_seed(args.seed)
@@ -171,7 +175,8 @@ def main(argv=None):
     kw = dict(image_id=args.image_id) if args.network == 'CIFAR' else {}
     res = fn(args.img_v, args.img_t, args.mask, args.lbl_v, args.lbl_t, args.pt_file, args.scorefile, args.heatmap,
              args.coarse_error, args.reduce_error, 1, args.mask_transforms, args.boost_transforms, net_size=32,
-             noise_size=32, joint_iters=args.joint_iters, checkpoint=ex.checkpoint, args=args,
+             noise_size=32, joint_iters=args.joint_iters, checkpoint=ex.checkpoint,
+             linear_w4=ex.linear_w4, args=args,
              write_outputs=not ex.no_outputs, **kw)
     print("\n\nTotal running time: %.4f seconds\n" % (time.time() - t0))
     return res

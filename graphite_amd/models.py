@@ -52,9 +52,31 @@ class _HipClassifier:
         self._require().set_precision(precision)
         return self
 
+    _linear = ("fc",)                # the state dict's linear layers, in gr_model_set_linear_w4's order
+
+    def set_linear_w4(self, layers):
+        """Runs linear layers on 4-bit weights: {name: linear_w4.LinearW4, or None for the float layer again}; names as in the
+        state dict (GTSRBNet: fc5_1, fc6_1, fc7_1; WideResNet: fc)."""
+        for name, layer in layers.items():
+            if name not in self._linear:
+                raise ValueError(f"no linear layer {name!r}; there are {', '.join(self._linear)}")
+            self._require().set_linear_w4(self._linear.index(name), layer)
+        return self
+
+    def quantize_linear(self, state_dict, group=64, symmetric=False, layers=None):
+        """The victim as a 4-bit deployment runs it: the linear layers of `state_dict` (the one the model was loaded from)
+        rounded to 4 bits with one scale per `group` inputs (linear_w4.quantize); `layers` limits it to some of them."""
+        from .linear_w4 import LinearW4, quantize
+        for name in layers or self._linear:
+            q, scales, zeros = quantize(state_dict[name + ".weight"], group, symmetric)
+            bias = torch.as_tensor(state_dict[name + ".bias"], dtype=torch.float32)
+            self.set_linear_w4({name: LinearW4(q, scales, zeros, bias=bias, group=group, in_features=int(state_dict[name + ".weight"].shape[1]))})
+        return self
+
 
 class GTSRBNet(_HipClassifier):
     num_classes = 43
+    _linear = ("fc5_1", "fc6_1", "fc7_1")
 
     def load_state_dict(self, state_dict, strict=True):
         self._model = _hip.Model("gtsrb", weights.gtsrb_tensor_list(state_dict))

@@ -87,9 +87,11 @@ def _remove_pixels(mask, grad, count):
 def whitebox_attack(model, img, mask, target_label, pt_file, num_xforms=100, step_size=0.0156862745, iters=50, min_tr=0.8,
                     gradient_shrink=False, aligned=True, patch_removal_size=-1, patch_removal_interval=15.25,
                     first_round_iters=500, max_rounds=None, xforms=None, verbose=False, patch_removal=True,
-                    pixels_per_round=5000, pixels_per_round_auto=True, model_type='GTSRB'):
+                    pixels_per_round=5000, pixels_per_round_auto=True, model_type='GTSRB', teacher=None):
     """img [3,H,W] in [0,1] (CPU or CUDA), mask [3,H,W] 0/1, model = graphite_amd.models.GTSRBNet (or WideResNet with
-    model_type='CIFAR').  Returns a dict: adversarial image and mask of the last round that reached `min_tr`, its
+    model_type='CIFAR').  teacher: a distill.TeacherTop; the gradient steps then follow the distillation loss against it
+    (engine.eot_gradient) instead of the cross entropy to `target_label`, which still decides the transform robustness.
+    Returns a dict: adversarial image and mask of the last round that reached `min_tr`, its
     transform robustness, mask size (pixels), query count, rounds."""
     normalize = model_type == 'GTSRB'                                       # :154-155
     dev = _hip.to_dev(img).device
@@ -115,7 +117,7 @@ def whitebox_attack(model, img, mask, target_label, pt_file, num_xforms=100, ste
         final_avg_grad, tr = None, 0.0
         loop_length = iters if rounds > 0 else first_round_iters           # :150
         for _ in range(loop_length):
-            avg_grad, _ = engine.eot_gradient(model, img, adv, mask, tab, target_label, normalize=normalize)
+            avg_grad, _ = engine.eot_gradient(model, img, adv, mask, tab, target_label, normalize=normalize, teacher=teacher)
             num_queries += T
             g = torch.nan_to_num(avg_grad, nan=0.0, posinf=float("inf"), neginf=float("-inf"))   # only NaN is zeroed (:164)
             if gradient_shrink:

@@ -36,8 +36,8 @@ def patch_positions(frame, mask_length, limited_loc=True, whole_attack_32=False)
 
 def whitebox_patch_attack(model, img, target_label, pt_file, mask_size, num_xforms=100, step_size=0.0156862745, iters=200,
                           limited_loc=True, gradient_shrink=False, whole_attack_32=False, xforms=None, model_type='GTSRB',
-                          verbose=False):
-    """img [3,H,H] in [0,1] (the 244 x 244 victim; with whole_attack_32 its 32 x 32 version).  Returns a dict: the best
+                          verbose=False, teacher=None):
+    """img [3,H,H] in [0,1] (the 244 x 244 victim; with whole_attack_32 its 32 x 32 version).  teacher: as whitebox_attack's.  Returns a dict: the best
     position's best iterate (`adversarial`), its mask, transform robustness and position, per-position results, and the
     number of classifier queries (2 T per iteration: gradient + evaluation)."""
     normalize = model_type == 'GTSRB'                                        # :161-162
@@ -56,7 +56,7 @@ def whitebox_patch_attack(model, img, target_label, pt_file, mask_size, num_xfor
         adv = torch.clamp(img.clone(), 0, 1)
         max_tr, best_img = -1, None
         for _ in range(iters):
-            avg_grad, _ = engine.eot_gradient(model, img, adv, mask, tab, target_label, normalize=normalize)
+            avg_grad, _ = engine.eot_gradient(model, img, adv, mask, tab, target_label, normalize=normalize, teacher=teacher)
             g = torch.nan_to_num(avg_grad, nan=0.0, posinf=float("inf"), neginf=float("-inf"))   # only NaN is zeroed (:166)
             if gradient_shrink and not whole_attack_32:
                 small = TREvaluator.resize(g.cpu(), 32, 32)

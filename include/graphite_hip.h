@@ -218,6 +218,19 @@ int gr_pg_masking_defense(gr_ctx* ctx, const float* local, int N, int h, int w, 
  * Always fp32, whatever gr_model_set_precision says. */
 int gr_model_input_grad(gr_ctx* ctx, gr_model* m, const float* x, int N, int target, float* logits, float* grad_x,
                         void* stream);
+/* The same gradient for a soft target (no counterpart in the reference, whose loss is the cross entropy to a label): grad_x =
+ * d loss_n / d x_n with loss_n = gr_distill_topk's loss of logits_n against the teacher's top classes (index, value, ld_top,
+ * teacher_lse, tau as there; value is float32).  loss [N] dev and logits [N,ncls] dev are optional. */
+int gr_model_input_grad_topk(gr_ctx* ctx, gr_model* m, const float* x, int N, const int64_t* index, const float* value, int k,
+                             int64_t ld_top, const float* teacher_lse, float tau, float* loss, float* logits, float* grad_x,
+                             void* stream);
+/* Runs a linear layer of the model on 4-bit weights (gr_w4_create, in_features in PyTorch's order): GTSRBNet layer 0 = fc5_1,
+ * 1 = fc6_1, 2 = fc7_1; WideResNet and BagNet layer 0 = fc.  Forward, predict, gr_tr_hits and the input gradients follow it;
+ * the activations stay float32 (GTSRBNet: GR_EINVAL together with GR_PREC_BF16).  w must have been created with input_grad if
+ * gradients are taken, belongs to the caller and must outlive its use; NULL puts the float layer back.  The logits of an image
+ * may differ in their last bits between batch sizes. */
+struct gr_w4;
+int gr_model_set_linear_w4(gr_model* m, int layer, const struct gr_w4* w);
 
 /* ---- fused TR evaluation --------------------------------------------------------------------
  * run_predictions(get_transformed_images(...)) for C candidates at once (utils.py:29-57):
