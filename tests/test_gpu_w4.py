@@ -81,6 +81,69 @@ def test_forward_and_gradient_match_float64(shape, dtype):
     _check_grad(layer, w, torch.randn((n, m), generator=g).to("cuda", dtype), gate)
 
 
+# More outputs than the few-row kernels take (12288 tiles of 16 x 16): the LDS-tiled kernel, with contractions of less than a
+# stage, of whole stages, with a ragged end, and groups that end inside, at and across its 64-step stages.
+MANY = [(1, 32), (31, 64), (64, 32), (64, 128), (129, 96), (200, 64), (320, 32), (321, 128), (512, 256), (385, 160), (450, 1024)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("depth,group", MANY, ids=["x".join(map(str, s)) for s in MANY])
+def test_many_rows_match_float64(depth, group, dtype):
+    i = MANY.index((depth, group))
+    g = torch.Generator().manual_seed(200 + i)
+    n, wide = 2100, 1610
+    layer, w, b = _layer(wide, depth, group, (F32, dtype, F16)[i % 3], zeros=i % 2 == 0, bias=i % 3 != 1, seed=50 + i)
+    _check_forward(layer, w, b, torch.randn((n, depth), generator=g).to("cuda", dtype), relu=i % 4 == 3)
+    layer, w, _ = _layer(depth, wide, group, (F32, dtype, F16)[i % 3], zeros=i % 2 == 0, seed=70 + i)
+    gate = torch.randn((n, wide), generator=g).to("cuda", dtype) if i % 2 else None
+    _check_grad(layer, w, torch.randn((n, depth), generator=g).to("cuda", dtype), gate)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+def test_many_strided_rows(dtype):
+    n, k, m = 2060, 1700, 1605                             # 129 x 107 and 129 x 101 tiles
+    layer, w, b = _layer(m, k, 64, bias=True, seed=3)
+    x = torch.full((n + 1, k + 3), float("nan"), device="cuda", dtype=dtype).as_strided((n, k), (k + 3, 1), 1)
+    x.copy_(torch.randn((n, k), generator=torch.Generator().manual_seed(5)))
+    obuf = torch.full((n + 2, m + 6), 7.0, device="cuda", dtype=dtype)
+    layer.forward(x, out=obuf[1:n + 1, 3:3 + m])
+    xd = x.double().cpu().numpy()
+    ref = R.linear(xd, w, b)
+    _check(obuf[1:n + 1, 3:3 + m], ref, _tol(ref, np.abs(xd) @ np.abs(w).T + np.abs(b), k + 64, dtype))
+    obuf[1:n + 1, 3:3 + m] = 7.0
+    assert bool((obuf == 7.0).all())
+    gy = torch.full((n + 1, m + 9), float("inf"), device="cuda", dtype=dtype).as_strided((n, m), (m + 9, 1), 3)
+    gy.copy_(torch.randn((n, m), generator=torch.Generator().manual_seed(6)))
+    xbuf = torch.full((n + 2, k + 5), 7.0, device="cuda", dtype=dtype)
+    layer.input_grad(gy, out=xbuf[1:n + 1, 2:2 + k])
+    gd = gy.double().cpu().numpy()
+    ref = R.input_grad(gd, w)
+    _check(xbuf[1:n + 1, 2:2 + k], ref, _tol(ref, np.abs(gd) @ np.abs(w), m + 64, dtype, 2.0 ** -15))
+    xbuf[1:n + 1, 2:2 + k] = 7.0
+    assert bool((xbuf == 7.0).all())
+
+
+def test_many_rows_runs_agree_and_replay():
+    layer, w, b = _layer(1610, 330, 64, bias=True, seed=13)
+    wide, _, _ = _layer(330, 1610, 64, seed=14)
+    x = torch.zeros((2100, 330), device="cuda", dtype=BF16)
+    y, gx = torch.empty((2100, 1610), device="cuda", dtype=BF16), torch.empty((2100, 1610), device="cuda", dtype=BF16)
+    layer.forward(x, out=y)
+    wide.input_grad(x, out=gx)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        layer.forward(x, relu=True, out=y)
+        wide.input_grad(x, gate=y, out=gx)
+    for i in range(3):
+        x.copy_(torch.randn((2100, 330), generator=torch.Generator().manual_seed(i)))
+        graph.replay()
+        torch.cuda.synchronize()
+        yw = layer.forward(x, relu=True)
+        assert torch.equal(y, yw) and torch.equal(gx, wide.input_grad(x, gate=yw))
+        torch.cuda.synchronize()
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
 @pytest.mark.parametrize("n", [1, 5, 40, 300])
 def test_strided_rows_and_untouched_surroundings(n, dtype):
@@ -124,7 +187,7 @@ def test_views_that_are_not_rows_are_copied():
     assert tuple(layer.forward(torch.randn(96, device="cuda")).shape) == (40,)
 
 
-@pytest.mark.parametrize("n", [3, 40, 300])
+@pytest.mark.parametrize("n", [3, 40, 300, 40000])
 @pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
 def test_infinities_stay_in_their_rows(dtype, n):
     """x[i,k] = inf gives +-inf by the sign of the weight and NaN for a weight of 0, as the formula says; other rows keep
@@ -151,7 +214,7 @@ def test_infinities_stay_in_their_rows(dtype, n):
     assert torch.equal(gx[keep], gbase[keep])
 
 
-@pytest.mark.parametrize("n", [2, 300])
+@pytest.mark.parametrize("n", [2, 300, 40000])
 def test_float32_extremes(n):
     """Activations near both ends of float32's range: the three-piece cut neither overflows nor loses its low pieces."""
     layer, w, b = _layer(33, 64, 32, zeros=False, seed=9)
