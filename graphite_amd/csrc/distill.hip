@@ -95,33 +95,44 @@ __device__ __forceinline__ kd_u32x4 kd_drop(kd_u32x4 r, unsigned bits) {
     return r;
 }
 
-// Reductions over the workgroup of two values at once; every thread gets the results.  `buf` holds two slots per wave.
-template <int NT, typename A, typename B, typename OA, typename OB>
-__device__ __forceinline__ void kd_reduce2(A& a, B& b, double* buf, OA oa, OB ob) {
+// Reductions over a wave, the result in every lane: floats by data-parallel moves (lane 63 collects), doubles by shuffles.
+template <typename OP>
+__device__ __forceinline__ float kd_wave(float x, float none, OP op) {
+    const int e = __float_as_int(none);
+#define KD_STEP(CTRL, ROWS) x = op(x, __int_as_float(__builtin_amdgcn_update_dpp(e, __float_as_int(x), CTRL, ROWS, 0xf, false)))
+    KD_STEP(0x111, 0xf);                                    // row_shr:1, 2, 4, 8
+    KD_STEP(0x112, 0xf);
+    KD_STEP(0x114, 0xf);
+    KD_STEP(0x118, 0xf);
+    KD_STEP(0x142, 0xa);                                    // row_bcast:15 into rows 1 and 3
+    KD_STEP(0x143, 0xc);                                    // row_bcast:31 into rows 2 and 3
+#undef KD_STEP
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+}
+template <typename OP>
+__device__ __forceinline__ double kd_wave(double x, OP op) {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        a = oa(a, __shfl_xor(a, o));
-        b = ob(b, __shfl_xor(b, o));
-    }
+    for (int o = 32; o > 0; o >>= 1) x = op(x, __shfl_xor(x, o));
+    return x;
+}
+// ... and over the workgroup; `slots` (one float per wave, 16-byte aligned) is not used again before the next barrier
+template <int NT, typename OP>
+__device__ __forceinline__ float kd_block(float x, float none, float* slots, OP op) {
+    x = kd_wave(x, none, op);
     if constexpr (NT > 64) {
-        if ((threadIdx.x & 63) == 0) {
-            buf[(threadIdx.x >> 6) * 2] = (double)a;
-            buf[(threadIdx.x >> 6) * 2 + 1] = (double)b;
-        }
+        if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = x;
         __syncthreads();
-        a = (A)buf[0];
-        b = (B)buf[1];
+        x = slots[0];
 #pragma unroll
-        for (int w = 1; w < NT / 64; w++) {
-            a = oa(a, (A)buf[w * 2]);
-            b = ob(b, (B)buf[w * 2 + 1]);
-        }
-        __syncthreads();
+        for (int w = 1; w < NT / 64; w++) x = op(x, slots[w]);
     }
+    return x;
 }
 
-// One workgroup per row.  VPT 16-byte vectors per thread of the row stay in registers between the pass that finds its maximum
-// and sum and the one that writes the gradient, so the row is read from memory once; what does not fit (BIG) is read again.
+// One workgroup per row.  VPT 16-byte vectors per thread of the row stay in registers between the pass that finds its maximum,
+// the one that sums and the one that writes the gradient, so the row is read from memory once; what does not fit (BIG) is read
+// again, mostly from the caches.  Bound by memory: 4096 x 32768 bf16 125 us = 4.3 TB/s, a copy of that size takes 100 us.
+// The teacher's few classes are the first wave's work.
 // LDS (dynamic): p [k] double | z [k] float | i [k] int | bits, one per class (OPEN), bit 32 = the first aligned element.
 template <int DT, int NT, int VPT, bool BIG, bool OPEN>
 __global__ __launch_bounds__(NT) void k_distill(KdParams p) {
@@ -129,7 +140,10 @@ __global__ __launch_bounds__(NT) void k_distill(KdParams p) {
     constexpr int VE = 16 / (int)sizeof(T);
     constexpr float NINF = -__builtin_inff();
     extern __shared__ __attribute__((aligned(16))) unsigned char kd_lds[];
-    __shared__ double s_red[2 * (NT / 64)];
+    __shared__ __attribute__((aligned(16))) float s_max[NT / 64], s_sum[NT / 64];
+    __shared__ int s_flags;
+    __shared__ float s_named, s_part;                       // maximum of the named logits, their sum of exp2
+    __shared__ double s_mass;                               // sum of the teacher's exp
     double* s_p = (double*)kd_lds;
     float* s_z = (float*)(s_p + p.k);
     int* s_i = (int*)(s_z + p.k);
@@ -148,12 +162,14 @@ __global__ __launch_bounds__(NT) void k_distill(KdParams p) {
     const int nv = (V - h) / VE, loose = V - nv * VE;
     const int li = tid < h ? tid : nv * VE + tid;
     const kd_u32x4* zv = (const kd_u32x4*)(z + h);
+    // vector tid + b of the row, b uniform: a scalar base and one 32-bit offset for all of a thread's vectors
+    const unsigned toff = (unsigned)tid * 16u;
+    const auto vec = [&](int b) { return *(const kd_u32x4*)((const char*)(zv + b) + toff); };
     kd_u32x4 r[VPT];
 #pragma unroll
     for (int v = 0; v < VPT; v++) {
-        const int i = tid + v * NT;
-        if (i < nv) r[v] = zv[i];
-        else r[v] = kd_drop<DT>(kd_u32x4{0, 0, 0, 0}, 0xffu);
+        r[v] = kd_drop<DT>(kd_u32x4{0, 0, 0, 0}, 0xffu);
+        if (tid < nv - v * NT) r[v] = vec(v * NT);
     }
     float lz = tid < loose ? (float)z[li] : NINF;
 
@@ -163,30 +179,46 @@ __global__ __launch_bounds__(NT) void k_distill(KdParams p) {
         for (int i = tid; i < (V - h + 63) / 32; i += NT) s_bits[i] = 0u;
         __syncthreads();
     }
-    const int64_t* ix = p.index + n * p.ld_top;
-    int flags = 0;                                          // 1: a slot is live, 2: a bad index, 4: a class may be named twice
-    double top = -__builtin_inf();
-    for (int j = tid; j < k; j += NT) {
-        const int64_t i = ix[j];
-        const double t = kd_value(p.value, p.vt, n * p.ld_top + j) / (double)p.tau;
-        const bool on = i >= 0 && i < V;
-        if (!on && i != -1) flags |= 2;
-        s_i[j] = on ? (int)i : -1;
-        s_z[j] = on ? (float)z[i] : 0.f;
-        s_p[j] = on ? t : -__builtin_inf();
-        if (on) {
-            if (bits) {
-                const int b = (int)i - h + 32;
-                if (atomicOr(&s_bits[b >> 5], 1u << (b & 31)) >> (b & 31) & 1u) flags |= 4;
-            } else {
-                flags |= 4;                                 // not known: compare them all
+    const bool first_wave = tid < 64;
+    if (first_wave) {
+        const int64_t* ix = p.index + n * p.ld_top;
+        int flags = 0;                                      // 1: a slot is live, 2: a bad index, 4: a class may be named twice
+        double top = -__builtin_inf();
+        for (int j = tid; j < k; j += 64) {
+            const int64_t i = ix[j];
+            const double t = kd_value(p.value, p.vt, n * p.ld_top + j) / (double)p.tau;
+            const bool on = i >= 0 && i < V;
+            if (!on && i != -1) flags |= 2;
+            s_i[j] = on ? (int)i : -1;
+            s_z[j] = on ? (float)z[i] : 0.f;
+            s_p[j] = on ? t : -__builtin_inf();
+            if (on) {
+                if (bits) {
+                    const int b = (int)i - h + 32;
+                    if (atomicOr(&s_bits[b >> 5], 1u << (b & 31)) >> (b & 31) & 1u) flags |= 4;
+                } else {
+                    flags |= 4;                             // not known: compare them all
+                }
+                if (OPEN || !(t == -__builtin_inf())) flags |= 1;
+                top = t > top ? t : top;
             }
-            if (OPEN || !(t == -__builtin_inf())) flags |= 1;
-            top = t > top ? t : top;
         }
+        flags = (__ballot(flags & 1) ? 1 : 0) | (__ballot(flags & 2) ? 2 : 0) | (__ballot(flags & 4) ? 4 : 0);
+        top = OPEN ? (double)p.lse[p.ld_top ? n : 0] : kd_wave(top, mx);
+        double sum = 0;
+        float mn = NINF;
+        for (int j = tid; j < k; j += 64) {
+            const double e = s_i[j] < 0 ? 0. : exp(s_p[j] - top);
+            s_p[j] = e;
+            sum += e;
+            if (OPEN && s_i[j] >= 0) mn = s_z[j] > mn ? s_z[j] : mn;
+        }
+        sum = kd_wave(sum, add);
+        mn = kd_wave(mn, NINF, mx);
+        if (tid == 0) { s_flags = flags; s_mass = sum; s_named = mn; }
     }
-    kd_reduce2<NT>(top, flags, s_red, mx, [](int a, int b) { return a | b; });
-    if (NT == 64) __syncthreads();                          // the slots, for the wave's other lanes
+    __syncthreads();
+    const int flags = s_flags;
     const float gl = p.grad_loss ? p.grad_loss[n] : 1.f;
     if ((flags & 2) || !(flags & 1)) {
         const float v = (flags & 2) ? __builtin_nanf("") : 0.f;
@@ -195,29 +227,26 @@ __global__ __launch_bounds__(NT) void k_distill(KdParams p) {
             for (int i = tid; i < V; i += NT) g[i] = (T)v;
         return;
     }
-    if (OPEN) top = (double)p.lse[p.ld_top ? n : 0];
-    double sum = 0;
-    float M = NINF;                                         // maximum of the named logits
-    for (int j = tid; j < k; j += NT) {
-        const double e = s_i[j] < 0 ? 0. : exp(s_p[j] - top);
-        s_p[j] = e;
-        sum += e;
-        if (OPEN && s_i[j] >= 0) M = s_z[j] > M ? s_z[j] : M;
-    }
 
     // ---- the unnamed classes: running maximum and sum of what is not kept, maximum of what is
-    const auto named = [&](int i) {                         // the bits of vector i
-        return VE == 8 ? (s_bits[(i >> 2) + 1] >> ((i & 3) * 8)) & 0xffu : (s_bits[(i >> 3) + 1] >> ((i & 7) * 4)) & 0xfu;
-    };
-    if (OPEN) {
+    constexpr int VW = 32 / VE;                              // vectors in a word of bits
+    static_assert(NT % VW == 0, "");
+    const int tw = tid / VW + 1, tb = tid % VW * VE;
+    const auto named = [&](int b) { return (s_bits[tw + b / VW] >> tb) & ((1u << VE) - 1u); };      // of vector tid + b
 #pragma unroll
-        for (int v = 0; v < VPT; v++) {
-            const int i = tid + v * NT;
-            if (i < nv) r[v] = kd_drop<DT>(r[v], named(i));
-        }
+    for (int v = 0; v < VPT; v++) {
+        if (OPEN && tid < nv - v * NT) r[v] = kd_drop<DT>(r[v], named(v * NT));
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    if (OPEN) {
         const int b = li - h + 32;
         if (tid < loose && (s_bits[b >> 5] >> (b & 31) & 1u)) lz = NINF;
     }
+    // Between the passes the vectors are made opaque: otherwise the compiler keeps their unpacked floats, twice the registers.
+    const auto forget = [&]() {
+#pragma unroll
+        for (int v = 0; v < VPT; v++) asm volatile("" : "+v"(r[v]));
+    };
     float m = lz;
 #pragma unroll
     for (int v = 0; v < VPT; v++) {
@@ -226,11 +255,12 @@ __global__ __launch_bounds__(NT) void k_distill(KdParams p) {
 #pragma unroll
         for (int e = 0; e < VE; e++) m = f[e] > m ? f[e] : m;
     }
+    forget();
     float bm = NINF, bs = 0.f;
     if (BIG) {
-        for (int i = tid + VPT * NT; i < nv; i += NT) {
-            kd_u32x4 q = zv[i];
-            if (OPEN) q = kd_drop<DT>(q, named(i));
+        for (int b = VPT * NT; tid < nv - b; b += NT) {
+            kd_u32x4 q = vec(b);
+            if (OPEN) q = kd_drop<DT>(q, named(b));
             float f[VE], mn = bm, t = 0.f;
             kd_unpack<DT>(q, f);
 #pragma unroll
@@ -243,21 +273,16 @@ __global__ __launch_bounds__(NT) void k_distill(KdParams p) {
         }
         m = bm > m ? bm : m;
     }
-    kd_reduce2<NT>(sum, m, s_red, add, mx);
-    const double inv = OPEN ? 1. : 1. / sum;
-    double rest = OPEN ? 1. - sum : 0.;
+    m = kd_block<NT>(m, NINF, s_max, mx);
+    const double mass = s_mass, inv = OPEN ? 1. : 1. / mass;
+    double rest = OPEN ? 1. - mass : 0.;
     if (rest < 0.) rest = 0.;
     const bool none = m == NINF;                            // no unnamed class, or none with a finite logit
     const float mr = none ? 0.f : m;
-    if (OPEN) {
-        float dummy = 0.f;
-        M = m > M ? m : M;
-        kd_reduce2<NT>(M, dummy, s_red, mx, add);
-    } else {
-        M = m;
-    }
+    const float named_max = s_named;
+    const float M = OPEN && named_max > m ? named_max : m;
 
-    float acc[VE], Sr = 0.f, part = 0.f;
+    float acc[VE], Sr = 0.f;
 #pragma unroll
     for (int e = 0; e < VE; e++) acc[e] = 0.f;
 #pragma unroll
@@ -266,19 +291,27 @@ __global__ __launch_bounds__(NT) void k_distill(KdParams p) {
         kd_unpack<DT>(r[v], f);
 #pragma unroll
         for (int e = 0; e < VE; e++) acc[e] += ex(f[e], mr);
+        __builtin_amdgcn_sched_barrier(0);
     }
+    forget();
 #pragma unroll
     for (int e = 0; e < VE; e++) Sr += acc[e];
     Sr += ex(lz, mr);
     if (BIG) Sr += bs * ex(bm, mr);
-    // merged probabilities: the first slot of a class takes them all, the others step back
-    for (int j = tid; j < k; j += NT) {
-        bool first = s_i[j] >= 0;
-        if (flags & 4)
-            for (int i = 0; i < j && first; i++) first = s_i[i] != s_i[j];
-        if (OPEN && first) part += ex(s_z[j], M);
+    if (OPEN && first_wave) {                               // every named class once
+        float part = 0.f;
+        for (int j = tid; j < k; j += 64) {
+            bool first = s_i[j] >= 0;
+            if (flags & 4)
+                for (int i = 0; i < j && first; i++) first = s_i[i] != s_i[j];
+            if (first) part += ex(s_z[j], M);
+        }
+        part = kd_wave(part, 0.f, add);
+        if (tid == 0) s_part = part;
     }
-    kd_reduce2<NT>(Sr, part, s_red, add, add);
+    Sr = kd_block<NT>(Sr, 0.f, s_sum, add);
+    if (NT == 64) __syncthreads();
+    const float part = OPEN ? s_part : 0.f;
     const float shift = none ? 0.f : ex(mr, M);
     const float St = part + Sr * shift;
     const bool tail = OPEN && !(rest <= 0.) && !(none && Sr == 0.f);
@@ -287,34 +320,35 @@ __global__ __launch_bounds__(NT) void k_distill(KdParams p) {
     if (g) {
         const bool same = (uintptr_t)(g + h) % 16 == 0;
         kd_u32x4* gv = (kd_u32x4*)(g + h);
-        const auto put = [&](int i, kd_u32x4 q) {
+        const auto put = [&](int b, kd_u32x4 q) {
             float f[VE];
             kd_unpack<DT>(q, f);
 #pragma unroll
             for (int e = 0; e < VE; e++) f[e] = A * ex(f[e], mr);
-            if (same) gv[i] = kd_packed<DT>(f);
+            if (same) *(kd_u32x4*)((char*)(gv + b) + toff) = kd_packed<DT>(f);
             else
 #pragma unroll
-                for (int e = 0; e < VE; e++) g[h + i * VE + e] = (T)f[e];
+                for (int e = 0; e < VE; e++) (g + h + (int64_t)b * VE)[tid * VE + e] = (T)f[e];
         };
 #pragma unroll
         for (int v = 0; v < VPT; v++) {
-            const int i = tid + v * NT;
-            if (i < nv) put(i, r[v]);
+            if (tid < nv - v * NT) put(v * NT, r[v]);
+            __builtin_amdgcn_sched_barrier(0);
         }
         if (BIG)
-            for (int i = tid + VPT * NT; i < nv; i += NT) {
-                kd_u32x4 q = zv[i];
-                if (OPEN) q = kd_drop<DT>(q, named(i));
-                put(i, q);
+            for (int b = VPT * NT; tid < nv - b; b += NT) {
+                kd_u32x4 q = vec(b);
+                if (OPEN) q = kd_drop<DT>(q, named(b));
+                put(b, q);
             }
         if (tid < loose) g[li] = (T)(A * ex(lz, mr));
     }
     __syncthreads();                                        // the named classes are written over; s_p is read across lanes
+    if (!first_wave) return;
     const double lnS = log((double)St);
     constexpr double LN2 = 0.69314718055994530942;
     double kl = 0;
-    for (int j = tid; j < k; j += NT) {
+    for (int j = tid; j < k; j += 64) {                     // the first slot of a class takes all its mass
         const int ij = s_i[j];
         bool first = ij >= 0;
         double pj = s_p[j];
@@ -329,8 +363,7 @@ __global__ __launch_bounds__(NT) void k_distill(KdParams p) {
         if (g) g[ij] = (T)(a0 * (__builtin_amdgcn_exp2f(d) / St - (float)pj));
     }
     if (p.loss) {
-        double dummy = 0;
-        kd_reduce2<NT>(kl, dummy, s_red, add, add);
+        kl = kd_wave(kl, add);
         if (tail) kl += rest * (log(rest) - (log((double)Sr) + (double)ex.arg(mr, M) * LN2 - lnS));
         if (tid == 0) p.loss[n] = (float)((double)p.tau * (double)p.tau * kl);
     }
@@ -350,12 +383,15 @@ hipError_t launch1(const KdParams& p, hipStream_t st) {
 template <int DT, bool OPEN>
 hipError_t launch(const KdParams& p, hipStream_t st) {
     const int64_t nv = (int64_t)p.V * (int64_t)sizeof(typename KdType<DT>::T) / 16;
+    // A row costs a workgroup four barriers and the first wave's work on the teacher's classes, so short rows take few waves
+    // (8192 rows of 2048 bf16: 64 threads 27 us, 256 45, 1024 146); long ones need loads in flight, and few rows many waves
+    // (4096 rows of 32768 bf16: 256 threads with the row in registers 125 us, 1024 130; 1 row of 131072 f32: 1024 threads 26 us,
+    // 256 66).  Rows beyond 64 KB are read twice rather than held by 1024 threads x 16 vectors, which spill (4096 x 32768 f32
+    // 238 us against 260, 515 x 100003 135 against 143).
     if (nv <= 64 * 4) return launch1<DT, 64, 4, false, OPEN>(p, st);
     if (nv <= 256 * 4) return launch1<DT, 256, 4, false, OPEN>(p, st);
-    if (nv <= 256 * 16) return launch1<DT, 256, 16, false, OPEN>(p, st);
-    if (nv <= 512 * 16) return launch1<DT, 512, 16, false, OPEN>(p, st);
-    if (nv <= 1024 * 16) return launch1<DT, 1024, 16, false, OPEN>(p, st);
-    return launch1<DT, 1024, 16, true, OPEN>(p, st);
+    if (nv <= 1024 * 4) return p.N >= 512 ? launch1<DT, 256, 16, false, OPEN>(p, st) : launch1<DT, 1024, 4, false, OPEN>(p, st);
+    return launch1<DT, 1024, 4, true, OPEN>(p, st);
 }
 
 }  // namespace

@@ -30,7 +30,7 @@ def topk_distill(logits, index, value, tau=1.0, teacher_lse=None, grad_loss=None
     Returns (loss float32 [N], grad [N, V] of logits' type = grad_loss[n] * d loss[n] / d logits[n], None without
     want_grad); grad_loss float32 [N] defaults to 1.  grad_out: optional result tensor, which may be `logits` itself."""
     z, ldz = _hip.float_rows(logits, "logits")
-    dev = z.device
+    dev, dt = z.device, z.dtype
     n, v = z.shape
     if index.dim() == 1:
         index = index[None]
@@ -38,29 +38,38 @@ def topk_distill(logits, index, value, tau=1.0, teacher_lse=None, grad_loss=None
         value = value[None]
     if index.dtype != torch.int64:
         raise _hip.GraphiteHipError(f"index has type {index.dtype}, expected int64")
-    if index.device != dev or index.dim() != 2 or index.shape != value.shape or index.shape[1] < 1:
+    rows, k = index.shape if index.dim() == 2 else (0, 0)
+    if index.device != dev or index.shape != value.shape or k < 1:
         raise _hip.GraphiteHipError(f"index {tuple(index.shape)} and value {tuple(value.shape)} must be [N, k] tensors on {dev}")
-    rows, k = index.shape
-    shared = rows == 1
-    if rows != n and not shared:
+    if rows != n and rows != 1:
         raise _hip.GraphiteHipError(f"index has {rows} rows, expected {n} or 1")
-    if value.device != dev or value.dtype not in _hip.DTYPES:
+    vt = _hip.DTYPES.get(value.dtype)
+    if value.device != dev or vt is None:
         raise _hip.GraphiteHipError(f"value must be a float32, bfloat16 or float16 tensor on {dev}")
     index, value = index.contiguous(), value.contiguous()
-    for name, t, size in (("teacher_lse", teacher_lse, rows), ("grad_loss", grad_loss, n)):
-        if t is not None and (t.device != dev or t.dtype != torch.float32 or t.numel() != size):
-            raise _hip.GraphiteHipError(f"{name} must be a float32 tensor of {size} elements on {dev}")
-    teacher_lse = None if teacher_lse is None else teacher_lse.contiguous()
-    grad_loss = None if grad_loss is None else grad_loss.contiguous()
+    lse_p = gl_p = grad_p = None
+    if teacher_lse is not None:
+        teacher_lse = _vector(teacher_lse, "teacher_lse", rows, dev)
+        lse_p = teacher_lse.data_ptr()
+    if grad_loss is not None:
+        grad_loss = _vector(grad_loss, "grad_loss", n, dev)
+        gl_p = grad_loss.data_ptr()
     loss = torch.empty((n,), device=dev, dtype=torch.float32)
     grad, ldg = None, v
     if grad_out is not None:
         grad, ldg = _hip.float_rows(grad_out, "grad_out", dev, v)
-        if grad is not grad_out or grad.dtype != z.dtype or grad.shape[0] != n:
-            raise _hip.GraphiteHipError(f"grad_out must be a {z.dtype} tensor [{n}, {v}] with the elements of a row next to each other")
+        if grad is not grad_out or grad.dtype != dt or grad.shape[0] != n:
+            raise _hip.GraphiteHipError(f"grad_out must be a {dt} tensor [{n}, {v}] with the elements of a row next to each other")
+        grad_p = grad.data_ptr()
     elif want_grad:
         grad = z.new_empty((n, v))
-    _hip.op_call("gr_distill_topk", dev, z.data_ptr(), _hip.DTYPES[z.dtype], n, v, ldz, index.data_ptr(), value.data_ptr(),
-                 _hip.DTYPES[value.dtype], k, 0 if shared else k, None if teacher_lse is None else teacher_lse.data_ptr(), float(tau),
-                 None if grad_loss is None else grad_loss.data_ptr(), loss.data_ptr(), None if grad is None else grad.data_ptr(), ldg)
+        grad_p = grad.data_ptr()
+    _hip.op_call("gr_distill_topk", dev, z.data_ptr(), _hip.DTYPES[dt], n, v, ldz, index.data_ptr(), value.data_ptr(), vt, k,
+                 0 if rows == 1 else k, lse_p, float(tau), gl_p, loss.data_ptr(), grad_p, ldg)
     return loss, grad
+
+
+def _vector(t, name, size, dev):
+    if t.device != dev or t.dtype != torch.float32 or t.numel() != size:
+        raise _hip.GraphiteHipError(f"{name} must be a float32 tensor of {size} elements on {dev}")
+    return t.contiguous()
