@@ -27,6 +27,7 @@ struct KdParams {
     int64_t N, ldz, ldg, ld_top;
     int V, k;
     float tau;
+    double inv_tau;
     float c_hi, c_lo;        // log2(e) / tau = c_hi + c_lo, both positive
     int bits;                // closed form: look for repeated classes with one bit per class (V <= 2^20)
 };
@@ -95,25 +96,29 @@ __device__ __forceinline__ kd_u32x4 kd_drop(kd_u32x4 r, unsigned bits) {
     return r;
 }
 
-// Reductions over a wave, the result in every lane: floats by data-parallel moves (lane 63 collects), doubles by shuffles.
-template <typename OP>
-__device__ __forceinline__ float kd_wave(float x, float none, OP op) {
-    const int e = __float_as_int(none);
-#define KD_STEP(CTRL, ROWS) x = op(x, __int_as_float(__builtin_amdgcn_update_dpp(e, __float_as_int(x), CTRL, ROWS, 0xf, false)))
-    KD_STEP(0x111, 0xf);                                    // row_shr:1, 2, 4, 8
-    KD_STEP(0x112, 0xf);
-    KD_STEP(0x114, 0xf);
-    KD_STEP(0x118, 0xf);
-    KD_STEP(0x142, 0xa);                                    // row_bcast:15 into rows 1 and 3
-    KD_STEP(0x143, 0xc);                                    // row_bcast:31 into rows 2 and 3
-#undef KD_STEP
-    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+// Reductions over a wave by data-parallel moves (lane 63 collects), the result in every lane.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float kd_move(float x, float none) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(none), __float_as_int(x), CTRL, ROWS, 0xf, false));
 }
-template <typename OP>
-__device__ __forceinline__ double kd_wave(double x, OP op) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) x = op(x, __shfl_xor(x, o));
-    return x;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double kd_move(double x, double none) {
+    return __hiloint2double(__builtin_amdgcn_update_dpp(__double2hiint(none), __double2hiint(x), CTRL, ROWS, 0xf, false),
+                            __builtin_amdgcn_update_dpp(__double2loint(none), __double2loint(x), CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ float kd_last(float x) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63)); }
+__device__ __forceinline__ double kd_last(double x) {
+    return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(x), 63), __builtin_amdgcn_readlane(__double2loint(x), 63));
+}
+template <typename F, typename OP>
+__device__ __forceinline__ F kd_wave(F x, F none, OP op) {
+    x = op(x, kd_move<0x111, 0xf>(x, none));                // row_shr:1, 2, 4, 8
+    x = op(x, kd_move<0x112, 0xf>(x, none));
+    x = op(x, kd_move<0x114, 0xf>(x, none));
+    x = op(x, kd_move<0x118, 0xf>(x, none));
+    x = op(x, kd_move<0x142, 0xa>(x, none));                // row_bcast:15 into rows 1 and 3
+    x = op(x, kd_move<0x143, 0xc>(x, none));                // row_bcast:31 into rows 2 and 3
+    return kd_last(x);
 }
 // ... and over the workgroup; `slots` (one float per wave, 16-byte aligned) is not used again before the next barrier
 template <int NT, typename OP>
@@ -186,7 +191,7 @@ __global__ __launch_bounds__(NT) void k_distill(KdParams p) {
         double top = -__builtin_inf();
         for (int j = tid; j < k; j += 64) {
             const int64_t i = ix[j];
-            const double t = kd_value(p.value, p.vt, n * p.ld_top + j) / (double)p.tau;
+            const double t = kd_value(p.value, p.vt, n * p.ld_top + j) * p.inv_tau;
             const bool on = i >= 0 && i < V;
             if (!on && i != -1) flags |= 2;
             s_i[j] = on ? (int)i : -1;
@@ -204,7 +209,7 @@ __global__ __launch_bounds__(NT) void k_distill(KdParams p) {
             }
         }
         flags = (__ballot(flags & 1) ? 1 : 0) | (__ballot(flags & 2) ? 2 : 0) | (__ballot(flags & 4) ? 4 : 0);
-        top = OPEN ? (double)p.lse[p.ld_top ? n : 0] : kd_wave(top, mx);
+        top = OPEN ? (double)p.lse[p.ld_top ? n : 0] : kd_wave(top, -__builtin_inf(), mx);
         double sum = 0;
         float mn = NINF;
         for (int j = tid; j < k; j += 64) {
@@ -213,7 +218,7 @@ __global__ __launch_bounds__(NT) void k_distill(KdParams p) {
             sum += e;
             if (OPEN && s_i[j] >= 0) mn = s_z[j] > mn ? s_z[j] : mn;
         }
-        sum = kd_wave(sum, add);
+        sum = kd_wave(sum, 0., add);
         mn = kd_wave(mn, NINF, mx);
         if (tid == 0) { s_flags = flags; s_mass = sum; s_named = mn; }
     }
@@ -363,7 +368,7 @@ __global__ __launch_bounds__(NT) void k_distill(KdParams p) {
         if (g) g[ij] = (T)(a0 * (__builtin_amdgcn_exp2f(d) / St - (float)pj));
     }
     if (p.loss) {
-        kl = kd_wave(kl, add);
+        kl = kd_wave(kl, 0., add);
         if (tail) kl += rest * (log(rest) - (log((double)Sr) + (double)ex.arg(mr, M) * LN2 - lnS));
         if (tid == 0) p.loss[n] = (float)((double)p.tau * (double)p.tau * kl);
     }
@@ -414,7 +419,7 @@ extern "C" int gr_distill_topk(gr_ctx* ctx, const void* z, int dtype, int64_t N,
     if (((uintptr_t)z | (uintptr_t)grad) % size(dtype) || (uintptr_t)value % size(value_type))
         return gr_fail(ctx, GR_EINVAL, "gr_distill_topk: misaligned tensor");
     if (grad == z && ldg != ldz) return gr_fail(ctx, GR_EINVAL, "gr_distill_topk: in place needs ldg == ldz");
-    KdParams p = {z, grad, index, value, value_type, teacher_lse, grad_loss, loss, N, ldz, ldg, ld_top, V, k, tau, 0, 0, V <= (1 << 20)};
+    KdParams p = {z, grad, index, value, value_type, teacher_lse, grad_loss, loss, N, ldz, ldg, ld_top, V, k, tau, 1.0 / (double)tau, 0, 0, V <= (1 << 20)};
     const double c = 1.4426950408889634074 / (double)tau;
     p.c_hi = (float)c;
     if ((double)p.c_hi >= c) p.c_hi = nextafterf(p.c_hi, 0.f);
