@@ -321,7 +321,10 @@ __global__ __launch_bounds__(NT) void k_distill(KdParams p) {
     const float St = part + Sr * shift;
     const bool tail = OPEN && !(rest <= 0.) && !(none && Sr == 0.f);
     const float a0 = gl * p.tau;
-    const float A = a0 * (shift / St - (tail ? (float)rest / Sr : 0.f));
+    // Unnamed gradients are a0 w_i / Sr (q_rest - p_rest): where the two are near 1, their difference is taken from what the
+    // named classes hold on either side, else directly.
+    const float q_rest = Sr * shift / St;
+    const float A = !tail ? a0 * (shift / St) : a0 / Sr * (rest > 0.5 ? (float)mass - part / St : q_rest - (float)rest);
     if (g) {
         const bool same = (uintptr_t)(g + h) % 16 == 0;
         kd_u32x4* gv = (kd_u32x4*)(g + h);
@@ -350,8 +353,7 @@ __global__ __launch_bounds__(NT) void k_distill(KdParams p) {
     }
     __syncthreads();                                        // the named classes are written over; s_p is read across lanes
     if (!first_wave) return;
-    const double lnS = log((double)St);
-    constexpr double LN2 = 0.69314718055994530942;
+    const double Ur = (double)Sr * (double)shift, lnS = log((double)part + Ur);
     double kl = 0;
     for (int j = tid; j < k; j += 64) {                     // the first slot of a class takes all its mass
         const int ij = s_i[j];
@@ -364,12 +366,13 @@ __global__ __launch_bounds__(NT) void k_distill(KdParams p) {
         if (!first) continue;
         pj *= inv;
         const float d = ex.arg(s_z[j], M);
-        if (pj > 0. || pj != pj) kl += pj * (log(pj) - ((double)d * LN2 - lnS));
+        if (pj > 0. || pj != pj) kl += pj * (log(pj) - (((double)s_z[j] - (double)M) * p.inv_tau - lnS));
         if (g) g[ij] = (T)(a0 * (__builtin_amdgcn_exp2f(d) / St - (float)pj));
     }
     if (p.loss) {
         kl = kd_wave(kl, 0., add);
-        if (tail) kl += rest * (log(rest) - (log((double)Sr) + (double)ex.arg(mr, M) * LN2 - lnS));
+        // log q_rest: as -log1p when it is near 0, where a difference of logarithms would lose it
+        if (tail) kl += rest * (log(rest) + (q_rest > 0.5f ? log1p((double)part / Ur) : lnS - (log((double)Sr) + ((double)mr - (double)M) * p.inv_tau)));
         if (tid == 0) p.loss[n] = (float)((double)p.tau * (double)p.tau * kl);
     }
 }
