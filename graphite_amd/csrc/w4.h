@@ -185,8 +185,12 @@ __device__ __forceinline__ typename W4Type<DT>::T w4_finish(const W4Params& p, f
 
 // ---------------------------------------------------------------------------------------------
 // Few rows.  A workgroup owns MT row tiles x NT tiles of 16 batch rows; its waves take the contraction's chunks in turn, D
-// chunks at a time (all their loads are issued before the first is used), and their sums meet in LDS, in wave order.
+// chunks at a time (all their loads are issued before the first is used), and their sums meet in LDS, in wave order: the long
+// axis is split inside the workgroup, so there is no workspace, no second launch and one order of summation.
 // Forward: GS = groups of a chunk (1, 2 or 4; 4 also where a border falls on any step).
+// One row is bound by the weights' bytes: the matrix unit pads it to 16 rows for nothing, and what costs is turning nibbles
+// into operands, 2.5 VALU instructions a weight.  8192 -> 8192 bf16, g = 128, one row: 10.9 us = 3.2 TB/s of weights (a copy
+// reaches 4.7).  2048 -> 1024 f32, 100 rows: 9.2 us a call, 10.3 us the kernel alone (its latency: two chunks a wave).
 // ---------------------------------------------------------------------------------------------
 constexpr int w4_rows_waves(int nt, bool) { return nt > 1 ? 8 : 16; }      // the most a workgroup may have
 template <int DT, int ST, int NT, int MT, int GS, int D, bool GRAD>
@@ -372,6 +376,12 @@ __global__ __launch_bounds__(w4_rows_waves(NT, GRAD) * 64) void k_w4_rows(W4Para
 // [16 bytes], the order the packed weights already have), so every LDS access is 64 lanes x 16 consecutive bytes.
 // Three LDS buffers, one barrier per stage: while a stage is multiplied, the next one's first operands are already read and
 // the one after is written, from registers that global memory filled a stage earlier.
+// Measured (4096 -> 4096, 4096 rows, bf16): 192 us = 715 TFLOP/s, a library product of that size 1220; its gradient at 2048 rows
+// 130 us = 530 (1060 of matrix work, two pieces); 8192 x 2048 -> 1024 f32 126 us = 272 (816 of matrix work; the f32 matrix
+// unit's peak is 157).  Nothing is saturated: the matrix unit is busy 29 % of the cycles (gradient 40), VALU issue takes 41,
+// LDS 29; two waves a SIMD, in step through the barrier, overlap them only in part.  Tried and slower: 4-wave workgroups of
+// 128 x 128 (251 us), halves of the waves taking turns at multiplying and staging (570 us), loads two stages ahead (no gain),
+// partial sums held over whole groups (219 us: 64 registers spilled), raised wave priority (+10 %).
 // ---------------------------------------------------------------------------------------------
 template <int DT, bool GRAD> struct W4Pieces {          // pieces of the weights and of the activations
     static constexpr int W = !GRAD ? 1 : DT == GR_DT_F32 ? 3 : 2;

@@ -64,7 +64,8 @@ class LinearW4:
     """gr_w4 handle: the weights laid out for the matrix units on one device.  q uint8 [out, ceil(in/2)], scales [out, G]
     (float32 / bfloat16 / float16, finite), zeros uint8 [out, G] or None, bias [out] or None; CPU tensors are moved to
     `device` (default: q's, or the current one).  in_features: the true number of inputs when it is odd.
-    input_grad=False drops the transposed copy that `input_grad` reads (half the memory)."""
+    input_grad=False drops the transposed copy that `input_grad` reads (half the memory).  The object's memory must outlive
+    what was captured with it: keep it as long as a HIP graph replays its calls."""
 
     def __init__(self, q, scales, zeros=None, bias=None, group=64, in_features=None, input_grad=True, device=None):
         self._h = C.c_void_p()
@@ -133,7 +134,7 @@ class LinearW4:
 
     def input_grad(self, grad_y, gate=None, out=None):
         """grad_y [..., out] -> d loss / d x [..., in] of its type; 0 where gate <= 0 (gate: the rectified activation the
-        layer read, shape of the result).  A ReLU of this layer is the caller's to apply to grad_y."""
+        layer read, shape of the result).  A ReLU of this layer is the caller's to apply to grad_y.  out: as forward's."""
         lead = None
         if grad_y.dim() != 2:
             lead = grad_y.shape[:-1]
