@@ -52,11 +52,19 @@ template <> struct W4Type<GR_DT_F16> { typedef _Float16 T; };
 __device__ __forceinline__ unsigned w4_pack_hi(float a, float b) {       // high halves of a (low) and b (high)
     return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
 }
+// Nibbles p and p + 4 of w as the halves 1024 + q of an f16 pair.  The constants sit in registers of both kinds, so that AND and
+// OR are one instruction.
+__device__ __forceinline__ unsigned w4_pair(unsigned w, int p) {
+    unsigned mask = 0x000f000fu, k = 0x64006400u;
+    asm("" : "+s"(mask));
+    asm("" : "+v"(k));
+    return ((w >> (4 * p)) & mask) | k;
+}
 // Two nibbles as float, minus z: nibbles p and p + 4 of w become the halves 1024 + q of an f16 pair (q sits in the lowest
 // mantissa bits), and one mixed-precision fma per element converts and subtracts.  Exact.
 __device__ __forceinline__ void w4_ints_f32(unsigned w, int p, float z0, float z1, float& a, float& b) {
     union { unsigned u; w4_f16x2 h; } c;
-    c.u = ((w >> (4 * p)) & 0x000f000fu) | 0x64006400u;
+    c.u = w4_pair(w, p);
     float one = 1.f;
     asm("" : "+s"(one));                                 // a factor the compiler cannot drop: it would convert and subtract in two steps
     a = __builtin_fmaf((float)c.h[0], one, -z0);
@@ -84,7 +92,7 @@ __device__ __forceinline__ w4_f16x8 w4_ints_f16(unsigned w, float zk) {
     const w4_f16x2 zz = {zh, zh};
 #pragma unroll
     for (int p = 0; p < 4; p++) {
-        o.u[p] = ((w >> (4 * p)) & 0x000f000fu) | 0x64006400u;
+        o.u[p] = w4_pair(w, p);
         o.h[p] = o.h[p] - zz;
     }
     return o.v;
