@@ -7,8 +7,9 @@
 //   forward   the matrix unit multiplies x by INTEGERS and a group's partial sum is scaled once, in f32:  no weight is ever
 //             rounded.  f32 activations are cut into three bf16 pieces (8 + 8 + 8 significand bits: the cut is exact), one
 //             matrix instruction each.
-//   gradient  the scale changes along the sum (it belongs to m), so it goes to gy: gy * s is formed in f32 and cut into two
-//             (16-bit types, 2^-17 relative) or three (f32, exact) bf16 pieces.
+//   gradient  the scale changes along the sum (it belongs to m), so it goes to a factor: to gy in the few-row kernel (gy * s in
+//             f32, its rows sharing one group), to the weights in the tiled one ((q - z) * s in f32, any mix of groups).  That
+//             factor is cut into two (16-bit types, 2^-15 relative: a 64th of their own rounding) or three (f32) bf16 pieces.
 // Sums are f32 throughout; only the stored output is rounded to the tensors' type.
 //
 // Packed layout ("tiles"): 16 rows x 128 contraction steps = 64 lanes x 16 bytes = 1 KB, the operand of four matrix
@@ -197,12 +198,12 @@ __device__ __forceinline__ typename W4Type<DT>::T w4_finish(const W4Params& p, f
 // axis is split inside the workgroup, so there is no workspace, no second launch and one order of summation.
 // Forward: GS = groups of a chunk (1, 2 or 4; 4 also where a border falls on any step).
 // One row is bound by the weights' bytes: the matrix unit pads it to 16 rows for nothing, and what costs is turning nibbles
-// into operands, 2.5 VALU instructions a weight.  8192 -> 8192 bf16, g = 128, one row: 10.9 us = 3.2 TB/s of weights (a copy
+// into operands, 2.5 VALU instructions a weight.  8192 -> 8192 bf16, g = 128, one row: 10.4 us = 3.4 TB/s of weights (a copy
 // reaches 4.7).  2048 -> 1024 f32, 100 rows: 9.2 us a call, 10.3 us the kernel alone (its latency: two chunks a wave).
 // ---------------------------------------------------------------------------------------------
-constexpr int w4_rows_waves(int nt, bool) { return nt > 1 ? 8 : 16; }      // the most a workgroup may have
+constexpr int w4_rows_waves(int nt) { return nt > 1 ? 8 : 16; }            // the most a workgroup may have
 template <int DT, int ST, int NT, int MT, int GS, int D, bool GRAD>
-__global__ __launch_bounds__(w4_rows_waves(NT, GRAD) * 64) void k_w4_rows(W4Params p) {
+__global__ __launch_bounds__(w4_rows_waves(NT) * 64) void k_w4_rows(W4Params p) {
     typedef typename W4Type<DT>::T T;
     extern __shared__ __attribute__((aligned(16))) float w4_red[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nwaves = blockDim.x >> 6;
@@ -409,6 +410,7 @@ struct W4Gemm {
     static_assert(BM / 16 * 64 % NT == 0 && X_ONE % NT == 0, "stage loads must divide evenly");
     static_assert(LDS <= 160 * 1024, "LDS");
     static_assert(GRAD || NT % (KS * BM) == 0, "one scale per thread and stage");
+    static_assert(KS == (!GRAD && P::X == 1 ? 2 : 1), "body16 takes two steps a stage, body one");
 };
 
 template <int DT, int ST, bool GRAD, int TM, int TN, int WM, int WN, int KS>
@@ -629,26 +631,25 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
         }
     };
 
-    // 64 contraction steps without borders: straight-line code.  Its matrix instructions are cut into slices of one row tile
-    // (TN of them), and the staging is dealt out over the slices, where it runs in the matrix unit's shadow.
-    // FIRST: the steps begin a group, FLUSH: they end one.  F holds the operands of the first step.
+    // Two stages (KS = 1: 64 contraction steps) without borders: straight-line code.  Its matrix instructions are cut into slices
+    // of one row tile (TN of them), and the staging is dealt out over the slices, where it runs in the matrix unit's shadow.
+    // FIRST: the steps begin a group, FLUSH: they end one.  fa[0], fx[0] hold the first step's operands, then the next pair's.
     Frag fa[2][P::W][TM], fx[2][P::X][TN];
-    auto read_a = [&](int f, const w4_u32x4* buf, int i) {
+    auto read_a = [&](int f, const w4_u32x4* buf) {
 #pragma unroll
         for (int q = 0; q < P::W; q++)
 #pragma unroll
-            for (int t = 0; t < TM; t++) fa[f][q][t].u = buf[q * G::A_ONE + ((wm * TM + t) * KS + i) * 64 + lane];
+            for (int t = 0; t < TM; t++) fa[f][q][t].u = buf[q * G::A_ONE + (wm * TM + t) * 64 + lane];
     };
-    auto read_x = [&](int f, const w4_u32x4* buf, int i) {
+    auto read_x = [&](int f, const w4_u32x4* buf) {
 #pragma unroll
         for (int q = 0; q < P::X; q++)
 #pragma unroll
-            for (int t = 0; t < TN; t++) fx[f][q][t].u = buf[P::W * G::A_ONE + q * G::X_ONE + ((wn * TN + t) * KS + i) * 64 + lane];
+            for (int t = 0; t < TN; t++) fx[f][q][t].u = buf[P::W * G::A_ONE + q * G::X_ONE + (wn * TN + t) * 64 + lane];
     };
     w4_u32x4 *b0 = w4_lds, *b1 = w4_lds + G::SLOTS, *b2 = w4_lds + 2 * G::SLOTS;      // stages s, s + 1, s + 2
     auto body = [&]<bool FIRST, bool FLUSH>(int s) {
-        constexpr int STEPS = 2 / KS * KS, NSL = KS * P::PROD * TM, NW = G::AV * KS, ITEMS = NW + 2 + 2 * G::XV;
-        static_assert(STEPS == 2, "");
+        constexpr int NSL = P::PROD * TM, NW = G::AV, ITEMS = NW + 2 + 2 * G::XV;
         auto mul = [&](int f, int qa, int qx, int t, int u, w4_f32x4 c) {
             if constexpr (F16OP) return w4_mfma(fa[f][qa][t].h, fx[f][qx][u].h, c);
             else return w4_mfma(fa[f][qa][t].b, fx[f][qx][u].b, c);
@@ -660,19 +661,16 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
 #pragma unroll
                 for (int r = 0; r < 4; r++) acc[t][u][r] = __builtin_fmaf(part[t][u][r], sc[t][r], acc[t][u][r]);
         };
-        int sl = 0;
 #pragma unroll
-        for (int f = 0; f < 2; f++) {                     // step f; its operands are fa[f], fx[f]
-            const int i = KS == 2 ? f : 0, st = s + (KS == 2 ? 0 : f);      // step of the stage, stage
-            if (KS == 1) sl = 0;
+        for (int f = 0; f < 2; f++) {                     // stage s + f; its operands are fa[f], fx[f]
+            int sl = 0;
             auto item = [&](int it) {
-                if (it < NW) store_w(b2, it / KS, it % KS);
+                if (it < NW) store_w(b2, it, 0);
                 else if (it == NW) store_sc(b2);
-                else if (it == NW + 1) load_w(st + 3);
+                else if (it == NW + 1) load_w(s + f + 3);
                 else if ((it - NW) % 2 == 0) store_x(b2, (it - NW - 2) / 2);
-                else xreg[(it - NW - 2) / 2].load(xrow[(it - NW - 2) / 2] + (st + 3) * KS * 32);
+                else xreg[(it - NW - 2) / 2].load(xrow[(it - NW - 2) / 2] + (s + f + 3) * 32);
             };
-            const bool wrap = i == KS - 1;                // the next step is the next stage's first
             int pr = 0;
 #pragma unroll
             for (int qa = 0; qa < P::W; qa++)
@@ -687,14 +685,14 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
                             if constexpr (GRAD) acc[t][u] = mul(f, qa, qx, t, u, acc[t][u]);
                             else part[t][u] = mul(f, qa, qx, t, u, FIRST && f == 0 && qx == 0 ? zero4 : part[t][u]);
                         }
-                        if (pr == 1 && t == 0) read_a(1 - f, wrap ? b1 : b0, wrap ? 0 : 1);
-                        if (pr == 1 && t == 1) read_x(1 - f, wrap ? b1 : b0, wrap ? 0 : 1);
+                        if (pr == 1 && t == 0) read_a(1 - f, b1);
+                        if (pr == 1 && t == 1) read_x(1 - f, b1);
 #pragma unroll
                         for (int it = 0; it < ITEMS; it++)
                             if (it * NSL / ITEMS == sl) item(it);
                         if constexpr (!GRAD && FLUSH) {
                             if (f == 1 && pr == P::PROD) {
-                                sc[t] = *(const w4_f32x4*)((const float*)(b0 + G::SC0) + (KS - 1) * G::BM + (wm * TM + t) * 16 + lh * 4);
+                                sc[t] = *(const w4_f32x4*)((const float*)(b0 + G::SC0) + (wm * TM + t) * 16 + lh * 4);
                                 if (t > 0) flush(t - 1);
                             }
                         }
@@ -702,13 +700,11 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
                         __builtin_amdgcn_sched_barrier(0);
                     }
                 }
-            if (wrap) {
-                if constexpr (!GRAD && FLUSH) {
-                    if (f == 1) flush(TM - 1);
-                }
-                __syncthreads();
-                w4_u32x4* t = b0; b0 = b1; b1 = b2; b2 = t;
+            if constexpr (!GRAD && FLUSH) {
+                if (f == 1) flush(TM - 1);
             }
+            __syncthreads();
+            w4_u32x4* t = b0; b0 = b1; b1 = b2; b2 = t;
         }
     };
 
@@ -792,22 +788,20 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
                 }
             crem = s * KS % p.gsteps;
         }
-    } else if (plain >= 2 / KS && (GRAD || p.gsteps % 2 == 0)) {
-        constexpr int D = 2 / KS;
-        read_a(0, b0, 0);
-        read_x(0, b0, 0);
+    } else if (plain >= 2 && (GRAD || p.gsteps % 2 == 0)) {
+        read_a(0, b0);
+        read_x(0, b0);
         if constexpr (GRAD) {
-            for (; s + D <= plain; s += D) body.template operator()<false, false>(s);
+            for (; s + 2 <= plain; s += 2) body.template operator()<false, false>(s);
         } else if (p.gsteps == 2) {
-            for (; s + D <= plain; s += D) body.template operator()<true, true>(s);
+            for (; s + 2 <= plain; s += 2) body.template operator()<true, true>(s);
         } else {
-            const int gst = p.gsteps / KS;
-            while (s + gst <= plain) {
-                const int e = s + gst - D;
+            while (s + p.gsteps <= plain) {
+                const int e = s + p.gsteps - 2;
                 body.template operator()<true, false>(s);
-                for (s += D; s < e; s += D) body.template operator()<false, false>(s);
+                for (s += 2; s < e; s += 2) body.template operator()<false, false>(s);
                 body.template operator()<false, true>(s);
-                s += D;
+                s += 2;
             }
         }
     }
@@ -861,7 +855,7 @@ template <int DT, int ST, int NT, int MT, int GS, bool GRAD>
 static hipError_t launch_rows(const W4Params& p, hipStream_t st) {
     constexpr int D = DT == GR_DT_F32 || NT > 1 || GRAD ? 1 : 2;
     const int64_t blocks = (int64_t)((p.R + 16 * MT - 1) / (16 * MT)) * ((p.N + 16 * NT - 1) / (16 * NT));
-    int waves = blocks >= 2048 ? 4 : blocks >= 512 ? 8 : w4_rows_waves(NT, GRAD);
+    int waves = blocks >= 2048 ? 4 : blocks >= 512 ? 8 : w4_rows_waves(NT);
     if (waves > p.chunks) waves = p.chunks;
     const size_t lds = (size_t)waves * MT * NT * 1024;
     auto kern = &k_w4_rows<DT, ST, NT, MT, GS, D, GRAD>;
