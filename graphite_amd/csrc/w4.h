@@ -137,13 +137,33 @@ template <int DT> struct W4Raw {
 #pragma unroll
         for (int i = 0; i < Q; i++) q[i] = *(const w4_u32x4_u*)(src + i * (16 / (int)sizeof(T)));
     }
-    // zero from `count` on (count <= 0: all); what is read there instead is the row's last element
-    __device__ __forceinline__ void load_part(const T* src, int count) {
-        union { w4_u32x4 q[Q]; T t[8]; } u;
+    // zero from `count` on (count <= 0: all).  The eight elements that end the row (there are eight: `wide`) take one load, like
+    // any others, and move down to their places: one load an element cost a product of 470 rows, 827 -> 3992 f16, 20 us of 52.
+    __device__ __forceinline__ void load_part(const T* src, int count, bool wide) {
+        union { w4_u32x4 q[Q]; T t[8]; unsigned u[4 * Q]; } u;
+        if (wide) {
+            load(count < 8 ? src + (count - 8) : src);
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const T v = src[e < count ? e : count - 1];
-            u.t[e] = e < count ? v : (T)0.f;
+            for (int i = 0; i < Q; i++) u.q[i] = q[i];
+            const int sh = count >= 8 ? 0 : 8 - count;                          // elements to move by; 8 and more leave nothing
+            constexpr int W = 4 / (int)sizeof(T);                               // elements of a dword
+#pragma unroll
+            for (int b = 4; b >= W; b >>= 1) {
+#pragma unroll
+                for (int i = 0; i < 4 * Q; i++) u.u[i] = sh & b ? (i + b / W < 4 * Q ? u.u[i + b / W] : 0u) : u.u[i];
+            }
+            if constexpr (W == 2) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) u.u[i] = sh & 1 ? __builtin_amdgcn_alignbit(i < 3 ? u.u[i + 1] : 0u, u.u[i], 16) : u.u[i];
+            }
+#pragma unroll
+            for (int i = 0; i < 4 * Q; i++) u.u[i] = sh >= 8 ? 0u : u.u[i];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const T v = src[e < count ? e : count - 1];                     // the row's last element
+                u.t[e] = e < count ? v : (T)0.f;
+            }
         }
 #pragma unroll
         for (int i = 0; i < Q; i++) q[i] = u.q[i];
@@ -179,17 +199,37 @@ __device__ __forceinline__ w4_f32x4 w4_mfma(w4_bf16x8 a, w4_bf16x8 b, w4_f32x4 c
 __device__ __forceinline__ w4_f32x4 w4_mfma(w4_f16x8 a, w4_f16x8 b, w4_f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
-// the sum v of output m of row n, through the epilogue, to memory
+// Outputs m .. m + 3 of row n, from their sums through the epilogue to memory.  They lie together in y: one store, which may
+// start at any element (four stores each cost a product of 6039 rows, 43 -> 3166 f16, half of 59 us).
+template <bool GRAD>
+__device__ __forceinline__ void w4_bias(const W4Params& p, int m, float (&bias)[4]) {
+#pragma unroll
+    for (int r = 0; r < 4; r++) bias[r] = !GRAD && p.bias ? p.bias[m + r < p.R ? m + r : p.R - 1] : 0.f;
+}
 template <int DT, bool GRAD>
-__device__ __forceinline__ typename W4Type<DT>::T w4_finish(const W4Params& p, float v, int64_t n, int m) {
+__device__ __forceinline__ void w4_put(const W4Params& p, w4_f32x4 sum, const float (&bias)[4], int64_t n, int m) {
     typedef typename W4Type<DT>::T T;
-    if constexpr (!GRAD) {
-        if (p.bias) v += p.bias[m];
-        if (p.relu) v = v < 0.f ? 0.f : v;
-    } else if (p.gate) {
-        v = (float)((const T*)p.gate)[n * p.ldg + m] > 0.f ? v : 0.f;
+    typedef unsigned V __attribute__((ext_vector_type(sizeof(T)), aligned(sizeof(T))));
+    union Four { T t[4]; V v; __device__ Four() {} } o;
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        float v = sum[r];
+        if constexpr (!GRAD) {
+            v += bias[r];
+            if (p.relu) v = v < 0.f ? 0.f : v;
+        } else if (p.gate) {
+            v = m + r < p.R && (float)((const T*)p.gate)[n * p.ldg + m + r] > 0.f ? v : 0.f;
+        }
+        o.t[r] = (T)v;
     }
-    return (T)v;
+    T* dst = (T*)p.y + n * p.ldy + m;
+    if (m + 4 <= p.R) {
+        *(V*)dst = o.v;
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            if (m + r < p.R) dst[r] = o.t[r];
+    }
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -199,13 +239,14 @@ __device__ __forceinline__ typename W4Type<DT>::T w4_finish(const W4Params& p, f
 // Forward: GS = groups of a chunk (1, 2 or 4; 4 also where a border falls on any step).
 // One row is bound by the weights' bytes: the matrix unit pads it to 16 rows for nothing, and what costs is turning nibbles
 // into operands, 2.5 VALU instructions a weight.  8192 -> 8192 bf16, g = 128, one row: 10.4 us = 3.4 TB/s of weights (a copy
-// reaches 4.7).  2048 -> 1024 f32, 100 rows: 9.2 us a call, 10.3 us the kernel alone (its latency: two chunks a wave).
+// reaches 4.7).  2048 -> 1024 f32, 100 rows: 8.1 us a call (its latency: two chunks a wave, then the join, in which a thread
+// adds and stores four outputs at once; one output a thread took 9.2).
 // ---------------------------------------------------------------------------------------------
 constexpr int w4_rows_waves(int nt) { return nt > 1 ? 8 : 16; }            // the most a workgroup may have
 template <int DT, int ST, int NT, int MT, int GS, int D, bool GRAD>
 __global__ __launch_bounds__(w4_rows_waves(NT) * 64) void k_w4_rows(W4Params p) {
     typedef typename W4Type<DT>::T T;
-    extern __shared__ __attribute__((aligned(16))) float w4_red[];
+    extern __shared__ __attribute__((aligned(16))) w4_f32x4 w4_red[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nwaves = blockDim.x >> 6;
     const int lr = lane & 15, lh = lane >> 4;
     const int nmt = (p.R + 16 * MT - 1) / (16 * MT);
@@ -246,7 +287,7 @@ __global__ __launch_bounds__(w4_rows_waves(NT) * 64) void k_w4_rows(W4Params p) 
 #pragma unroll
             for (int i = 0; i < 4; i++)
 #pragma unroll
-                for (int t = 0; t < NT; t++) h.x[i][t].load_part(xrow[t] + kb + i * 32, p.C - kb - i * 32 - lh * 8);
+                for (int t = 0; t < NT; t++) h.x[i][t].load_part(xrow[t] + kb + i * 32, p.C - kb - i * 32 - lh * 8, p.C >= 8);
         }
         if constexpr (!GRAD) {
 #pragma unroll
@@ -358,23 +399,21 @@ __global__ __launch_bounds__(w4_rows_waves(NT) * 64) void k_w4_rows(W4Params p) 
             mul(h);
         }
 
-    // [wave][tile][reg][lane]
+    // [wave][tile][lane]: four sums; the threads add over the waves, in their order
 #pragma unroll
     for (int a = 0; a < MT; a++)
 #pragma unroll
-        for (int t = 0; t < NT; t++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) w4_red[(((wave * MT + a) * NT + t) * 4 + r) * 64 + lane] = acc[a][t][r];
+        for (int t = 0; t < NT; t++) w4_red[((wave * MT + a) * NT + t) * 64 + lane] = acc[a][t];
     __syncthreads();
-    for (int o = threadIdx.x; o < NT * 16 * MT * 16; o += blockDim.x) {
-        const int mm = o % (MT * 16), nn = o / (MT * 16);
-        const int64_t n = n0 + nn;
-        const int m = rt0 * 16 + mm;
+    for (int o = threadIdx.x; o < MT * NT * 64; o += blockDim.x) {
+        const int64_t n = n0 + (o / 64 % NT) * 16 + lr;
+        const int m = (rt0 + o / (64 * NT)) * 16 + lh * 4;
         if (n >= p.N || m >= p.R) continue;
-        const int src = (((mm >> 4) * NT + (nn >> 4)) * 4 + (mm & 3)) * 64 + ((mm >> 2) & 3) * 16 + (nn & 15);
-        float v = 0.f;
-        for (int w = 0; w < nwaves; w++) v += w4_red[w * (MT * NT * 256) + src];
-        ((T*)p.y)[n * p.ldy + m] = w4_finish<DT, GRAD>(p, v, n, m);
+        w4_f32x4 v = w4_red[o];
+        for (int w = 1; w < nwaves; w++) v += w4_red[w * (MT * NT * 64) + o];
+        float bias[4];
+        w4_bias<GRAD>(p, m, bias);
+        w4_put<DT, GRAD>(p, v, bias, n, m);
     }
 }
 
@@ -498,7 +537,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
             for (int v = 0; v < G::XV; v++) xreg[v].load(xrow[v] + s * KS * 32);
         } else {
 #pragma unroll
-            for (int v = 0; v < G::XV; v++) xreg[v].load_part(xrow[v] + s * KS * 32, p.C - s * KS * 32 - xk[v]);
+            for (int v = 0; v < G::XV; v++) xreg[v].load_part(xrow[v] + s * KS * 32, p.C - s * KS * 32 - xk[v], p.C >= 8);
         }
     };
     union Frag { w4_u32x4 u; w4_bf16x8 b; w4_f16x8 h; };
@@ -819,26 +858,15 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
         w4_u32x4* t = b0; b0 = b1; b1 = b2; b2 = t;
     }
 
-    const bool vec = ((uintptr_t)p.y % (4 * sizeof(T)) == 0) && p.ldy % 4 == 0;
 #pragma unroll
-    for (int u = 0; u < TN; u++) {
-        const int64_t n = n0 + (wn * TN + u) * 16 + lr;
-        if (n >= p.N) continue;
+    for (int t = 0; t < TM; t++) {
+        const int m = m0 + (wm * TM + t) * 16 + lh * 4;
+        float bias[4];
+        w4_bias<GRAD>(p, m, bias);
 #pragma unroll
-        for (int t = 0; t < TM; t++) {
-            const int m = m0 + (wm * TM + t) * 16 + lh * 4;
-            T v[4];
-#pragma unroll
-            for (int r = 0; r < 4; r++) v[r] = m + r < p.R ? w4_finish<DT, GRAD>(p, acc[t][u][r], n, m + r) : (T)0.f;
-            T* dst = (T*)p.y + n * p.ldy + m;
-            if (vec && m + 4 <= p.R) {
-                struct alignas(4 * sizeof(T)) T4 { T t[4]; } o = {{v[0], v[1], v[2], v[3]}};
-                *(T4*)dst = o;
-            } else {
-#pragma unroll
-                for (int r = 0; r < 4; r++)
-                    if (m + r < p.R) dst[r] = v[r];
-            }
+        for (int u = 0; u < TN; u++) {
+            const int64_t n = n0 + (wn * TN + u) * 16 + lr;
+            if (n < p.N && m < p.R) w4_put<DT, GRAD>(p, acc[t][u], bias, n, m);
         }
     }
 }
