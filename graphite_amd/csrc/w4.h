@@ -913,24 +913,64 @@ static hipError_t launch_gemm(const W4Params& p, hipStream_t st) {
 }
 template <int DT, int ST, bool GRAD>
 static hipError_t launch_typed(const W4Params& p, hipStream_t st) {
-    // Few rows: the smallest tile that leaves at most one workgroup a CU.  A workgroup's time depends on its tile and on the
-    // contraction, hardly on how many there are: 4096 -> 4096 bf16, g = 128, row tiles x batch tiles 1x1 7.5 us, 2x1 9.8, 2x2 14,
-    // 4x2 19, 4x4 30 (gradient 2x1 14, 4x1 20, 4x2 25, 8x2 37).  Many rows: the tiled kernel, whose one round of workgroups
-    // takes 90 us there (f32 110 us; gradient 127 us) and covers 32768 tiles (f32 and f16 gradient 16384).
-    const int64_t tiles = (int64_t)((p.R + 15) / 16) * ((p.N + 15) / 16);        // of 16 x 16 outputs
+    // A variant's time is about that of one workgroup, which grows with the contraction, times the rounds that its workgroups
+    // need:  max(1, workgroups / at_once) * (fixed + chunk * chunks)  microseconds, fitted to the variants' times at 1400 sizes (17
+    // to 8192 rows, 33 to 8192 on both sides, every group).  The variant with the least estimate takes 3 to 5 % longer than the
+    // fastest one (geometric mean); limits on the number of output tiles took 5 to 9 % and up to 2.3 times as long.
+    // Small tiles carry short contractions and few rows, the tiled kernel large products (us, in the order of `fwd`):  bf16,
+    // 320 rows 96 -> 6528  10.7 8.4 9.3 10.3 14.4 11.5;  f32, 384 rows 7680 -> 2848  -, -, 169 122 217 184;  bf16, 2464 rows
+    // 3648 -> 2048  -, -, 159 110 138 81.
+    struct Cost { float fixed, chunk, at_once; };
+    constexpr bool F32 = DT == GR_DT_F32, F16 = DT == GR_DT_F16;
+    constexpr Cost fwd[6] = {F32 ? Cost{0.05f, 0.18f, 197.f} : Cost{0.05f, 0.09f, 184.f},      // row tiles x batch tiles: 1 x 1
+                             F32 ? Cost{0.05f, 0.22f, 180.f} : Cost{0.05f, 0.11f, 151.f},      // 2 x 1
+                             F32 ? Cost{0.11f, 0.46f, 172.f} : Cost{0.15f, 0.23f, 184.f},      // 2 x 2
+                             F32 ? Cost{0.36f, 0.59f, 154.f} : Cost{0.33f, 0.35f, 169.f},      // 4 x 2
+                             F32 ? Cost{3.82f, 1.68f, 223.f} : Cost{3.77f, 0.57f, 218.f},      // 4 x 4
+                             F32 ? Cost{0.05f, 2.87f, 154.f} : Cost{0.79f, 2.87f, 125.f}};     // tiled
+    constexpr Cost grad[5] = {F32 ? Cost{0.05f, 0.29f, 182.f} : Cost{0.05f, 0.21f, 176.f},     // 2 x 1
+                              F32 ? Cost{0.06f, 0.34f, 184.f} : Cost{0.05f, 0.29f, 183.f},     // 4 x 1
+                              F32 ? Cost{0.16f, 0.70f, 172.f} : Cost{0.28f, 0.55f, 183.f},     // 4 x 2
+                              F32 ? Cost{1.42f, 1.00f, 200.f} : Cost{1.86f, 0.78f, 218.f},     // 8 x 2
+                              F32 ? Cost{0.05f, 4.16f, 143.f} : F16 ? Cost{0.05f, 3.02f, 148.f} : Cost{0.05f, 3.24f, 118.f}};  // tiled
+    auto time = [&](const Cost& c, int rows, int cols, float slower) {          // of workgroups of rows x cols outputs
+        const float blocks = (float)((p.R + rows - 1) / rows) * (float)((p.N + cols - 1) / cols);
+        return (blocks > c.at_once ? blocks / c.at_once : 1.f) * (c.fixed + c.chunk * slower * (float)p.chunks);
+    };
+    constexpr int tiled_cols = F32 || (GRAD && F16) ? 128 : 256;
+    int best = 0;
+    float least = 3e38f;
+    auto consider = [&](int i, float t) {
+        if (t < least) { least = t; best = i; }
+    };
     if constexpr (!GRAD) {
-        if (tiles <= 256) return launch_rows<DT, ST, 1, 1, GRAD>(p, st);
-        if (p.N <= 16 || tiles <= 512) return launch_rows<DT, ST, 1, 2, GRAD>(p, st);
-        if (tiles <= 1024) return launch_rows<DT, ST, 2, 2, GRAD>(p, st);
-        if (tiles <= 2048) return launch_rows<DT, ST, 2, 4, GRAD>(p, st);
-        if (tiles <= (DT == GR_DT_F32 ? 6144 : 12288)) return launch_rows<DT, ST, 4, 4, GRAD>(p, st);
-    } else if (p.N <= 16 || tiles <= 12288) {
+        consider(0, time(fwd[0], 16, 16, 1.f));
+        consider(1, time(fwd[1], 32, 16, 1.f));
+        if (p.N > 16) {
+            consider(2, time(fwd[2], 32, 32, 1.f));
+            consider(3, time(fwd[3], 64, 32, 1.f));
+            consider(4, time(fwd[4], 64, 64, 1.f));
+            consider(5, time(fwd[5], 128, tiled_cols, p.gsteps % 2 ? 1.3f : 1.f));     // groups of odd multiples of 32: more partial sums
+        }
+        if (best == 0) return launch_rows<DT, ST, 1, 1, GRAD>(p, st);
+        if (best == 1) return launch_rows<DT, ST, 1, 2, GRAD>(p, st);
+        if (best == 2) return launch_rows<DT, ST, 2, 2, GRAD>(p, st);
+        if (best == 3) return launch_rows<DT, ST, 2, 4, GRAD>(p, st);
+        if (best == 4) return launch_rows<DT, ST, 4, 4, GRAD>(p, st);
+    } else {
         // a workgroup's row tiles share one group: its scales go to the activations
         const int most = p.gsteps % 4 == 0 ? 8 : p.gsteps % 2 == 0 ? 4 : 2;
-        if (p.N <= 16 || tiles <= 512 || most == 2) return launch_rows<DT, ST, 1, 2, GRAD>(p, st);
-        if (tiles <= 1024) return launch_rows<DT, ST, 1, 4, GRAD>(p, st);
-        if (tiles <= 2048 || most == 4) return launch_rows<DT, ST, 2, 4, GRAD>(p, st);
-        return launch_rows<DT, ST, 2, 8, GRAD>(p, st);
+        consider(0, time(grad[0], 32, 16, 1.f));
+        if (most >= 4) consider(1, time(grad[1], 64, 16, 1.f));
+        if (p.N > 16) {
+            if (most >= 4) consider(2, time(grad[2], 64, 32, 1.f));
+            if (most == 8) consider(3, time(grad[3], 128, 32, 1.f));
+            consider(4, time(grad[4], 128, tiled_cols, 1.f));
+        }
+        if (best == 0) return launch_rows<DT, ST, 1, 2, GRAD>(p, st);
+        if (best == 1) return launch_rows<DT, ST, 1, 4, GRAD>(p, st);
+        if (best == 2) return launch_rows<DT, ST, 2, 4, GRAD>(p, st);
+        if (best == 3) return launch_rows<DT, ST, 2, 8, GRAD>(p, st);
     }
     if constexpr (DT == GR_DT_F32 || (GRAD && DT == GR_DT_F16)) return launch_gemm<DT, ST, GRAD, 4, 2, 2, 4, 1>(p, st);
     else if constexpr (GRAD) return launch_gemm<DT, ST, GRAD, 4, 4, 2, 4, 1>(p, st);
