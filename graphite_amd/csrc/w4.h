@@ -126,23 +126,55 @@ __device__ __forceinline__ void w4_pieces(const float (&v)[8], w4_bf16x8 (&out)[
 }
 
 // Eight consecutive elements of a row, as loaded.  Rows need no alignment beyond their elements' (the hardware takes 16-byte
-// loads at any element).
-typedef unsigned w4_u32x4_u __attribute__((ext_vector_type(4), aligned(2)));
-typedef unsigned w4_u32x2_u __attribute__((ext_vector_type(2), aligned(2)));
-template <int DT> struct W4Raw {
+// loads at any dword).  HALF: rows of 16-bit elements that may begin in the middle of a dword, where a 16-byte load takes
+// several times as long.  Whole dwords are loaded instead, a fifth one with the last half, and `settle` moves the elements down
+// before they are used; every dword read holds an element of the row.  2048 rows 4095 -> 4096 bf16: 226 us with the long loads,
+// 126 so (4096 -> 4096: 100).
+typedef unsigned w4_u32x4_u __attribute__((ext_vector_type(4), aligned(4)));
+template <int DT, bool HALF = false> struct W4Raw {
     static constexpr int Q = DT == GR_DT_F32 ? 2 : 1;
     typedef typename W4Type<DT>::T T;
+    static_assert(!HALF || sizeof(T) == 2, "only 16-bit elements begin in the middle of a dword");
     w4_u32x4 q[Q];
+    unsigned fifth[1];
     __device__ __forceinline__ void load(const T* src) {
+        if constexpr (HALF) {
+            const bool mid = (uintptr_t)src & 2;
+            const unsigned* d = (const unsigned*)(src - (mid ? 1 : 0));
+            q[0] = *(const w4_u32x4_u*)d;
+            fifth[0] = d[mid ? 4 : 3];
+        } else {
 #pragma unroll
-        for (int i = 0; i < Q; i++) q[i] = *(const w4_u32x4_u*)(src + i * (16 / (int)sizeof(T)));
+            for (int i = 0; i < Q; i++) q[i] = *(const w4_u32x4_u*)(src + i * (16 / (int)sizeof(T)));
+        }
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < Q; i++) q[i] = w4_u32x4{0u, 0u, 0u, 0u};
+        fifth[0] = 0u;
+    }
+    // HALF: mid = 16 where the row begins in the middle of a dword, 0 elsewhere
+    __device__ __forceinline__ void settle(unsigned mid) {
+        if constexpr (HALF) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) q[0][i] = __builtin_amdgcn_alignbit(i < 3 ? q[0][i + 1] : fifth[0], q[0][i], mid);
+        }
+    }
+    __device__ __forceinline__ void unsettle(unsigned mid) {
+        if constexpr (HALF) {
+            fifth[0] = q[0][3] >> 16;
+#pragma unroll
+            for (int i = 3; i >= 0; i--) q[0][i] = mid ? __builtin_amdgcn_alignbit(q[0][i], i > 0 ? q[0][i - 1] : 0u, 16) : q[0][i];
+        }
     }
     // zero from `count` on (count <= 0: all).  The eight elements that end the row (there are eight: `wide`) take one load, like
     // any others, and move down to their places: one load an element cost a product of 470 rows, 827 -> 3992 f16, 20 us of 52.
     __device__ __forceinline__ void load_part(const T* src, int count, bool wide) {
         union { w4_u32x4 q[Q]; T t[8]; unsigned u[4 * Q]; } u;
         if (wide) {
-            load(count < 8 ? src + (count - 8) : src);
+            const T* from = count < 8 ? src + (count - 8) : src;
+            load(from);
+            settle((uintptr_t)from & 2 ? 16 : 0);
 #pragma unroll
             for (int i = 0; i < Q; i++) u.q[i] = q[i];
             const int sh = count >= 8 ? 0 : 8 - count;                          // elements to move by; 8 and more leave nothing
@@ -167,6 +199,7 @@ template <int DT> struct W4Raw {
         }
 #pragma unroll
         for (int i = 0; i < Q; i++) q[i] = u.q[i];
+        unsettle((uintptr_t)src & 2 ? 16 : 0);
     }
     __device__ __forceinline__ void get(float (&f)[8]) const {
         if constexpr (DT == GR_DT_F32) {
@@ -243,7 +276,7 @@ __device__ __forceinline__ void w4_put(const W4Params& p, w4_f32x4 sum, const fl
 // adds and stores four outputs at once; one output a thread took 9.2).
 // ---------------------------------------------------------------------------------------------
 constexpr int w4_rows_waves(int nt) { return nt > 1 ? 8 : 16; }            // the most a workgroup may have
-template <int DT, int ST, int NT, int MT, int GS, int D, bool GRAD>
+template <int DT, int ST, bool HALF, int NT, int MT, int GS, int D, bool GRAD>
 __global__ __launch_bounds__(w4_rows_waves(NT) * 64) void k_w4_rows(W4Params p) {
     typedef typename W4Type<DT>::T T;
     extern __shared__ __attribute__((aligned(16))) w4_f32x4 w4_red[];
@@ -253,10 +286,12 @@ __global__ __launch_bounds__(w4_rows_waves(NT) * 64) void k_w4_rows(W4Params p) 
     const int rt0 = (int)(blockIdx.x % nmt) * MT;
     const int64_t n0 = (int64_t)(blockIdx.x / nmt) * (16 * NT);
     const T* xrow[NT];
+    unsigned mid[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) {
         const int64_t n = n0 + t * 16 + lr;
         xrow[t] = (const T*)p.x + (n < p.N ? n : p.N - 1) * p.ldx + lh * 8;      // columns beyond the batch: computed, not stored
+        mid[t] = (uintptr_t)xrow[t] & 2 ? 16 : 0;
     }
     const size_t grow = GRAD ? (size_t)((rt0 >> 1) / p.gsteps) * p.Mp : 0;        // the rows' one group
     const size_t zrow = GRAD ? (size_t)((rt0 >> 1) / p.gsteps) * p.zstride : 0;
@@ -268,7 +303,7 @@ __global__ __launch_bounds__(w4_rows_waves(NT) * 64) void k_w4_rows(W4Params p) 
 
     struct Chunk {
         w4_u32x4 w[MT];
-        W4Raw<DT> x[4][NT];
+        W4Raw<DT, HALF> x[4][NT];
         W4Scale4<ST> s[GRAD ? 1 : GS][MT];
         uint8_t z[GRAD ? 1 : GS][MT];
         W4Raw<ST> gs[GRAD ? 4 : 1];
@@ -287,7 +322,11 @@ __global__ __launch_bounds__(w4_rows_waves(NT) * 64) void k_w4_rows(W4Params p) 
 #pragma unroll
             for (int i = 0; i < 4; i++)
 #pragma unroll
-                for (int t = 0; t < NT; t++) h.x[i][t].load_part(xrow[t] + kb + i * 32, p.C - kb - i * 32 - lh * 8, p.C >= 8);
+                for (int t = 0; t < NT; t++) {
+                    if (kb + i * 32 + 32 <= p.C) h.x[i][t].load(xrow[t] + kb + i * 32);
+                    else if (kb + i * 32 < p.C) h.x[i][t].load_part(xrow[t] + kb + i * 32, p.C - kb - i * 32 - lh * 8, p.C >= 8);
+                    else h.x[i][t].clear();
+                }
         }
         if constexpr (!GRAD) {
 #pragma unroll
@@ -310,7 +349,11 @@ __global__ __launch_bounds__(w4_rows_waves(NT) * 64) void k_w4_rows(W4Params p) 
             }
         }
     };
-    auto mul = [&](const Chunk& h) {
+    auto mul = [&](Chunk& h) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int t = 0; t < NT; t++) h.x[i][t].settle(mid[t]);
         if constexpr (!GRAD) {
 #pragma unroll
             for (int g = 0; g < GS; g++) {
@@ -452,7 +495,7 @@ struct W4Gemm {
     static_assert(KS == (!GRAD && P::X == 1 ? 2 : 1), "body16 takes two steps a stage, body one");
 };
 
-template <int DT, int ST, bool GRAD, int TM, int TN, int WM, int WN, int KS>
+template <int DT, int ST, bool HALF, bool GRAD, int TM, int TN, int WM, int WN, int KS>
 __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
     using G = W4Gemm<DT, GRAD, TM, TN, WM, WN, KS>;
     using P = typename G::P;
@@ -471,7 +514,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
 
     // ---- staging: thread's share of the weights (AV packed lanes) and of the activations (XV runs of eight)
     unsigned wreg[G::AV][KS];
-    W4Raw<DT> xreg[G::XV];
+    W4Raw<DT, HALF> xreg[G::XV];
     uint8_t zreg[GRAD ? 1 : G::AV][KS];
     W4Raw<ST> sreg[GRAD ? G::AV : 1][KS];                 // GRAD: scales and zeros run along the steps
     uint2 szreg[GRAD ? G::AV : 1][KS];
@@ -571,6 +614,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
     };
     auto store_x = [&](w4_u32x4* buf, int v) {
         w4_u32x4* dst = buf + P::W * G::A_ONE + tid + v * G::NT;
+        xreg[v].settle((uintptr_t)xrow[v] & 2 ? 16 : 0);
         if constexpr (P::X == 1) {
             dst[0] = xreg[v].q[0];
         } else {
@@ -872,21 +916,24 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// launchers (one translation unit per activation type: w4_f32.hip, w4_bf16.hip, w4_f16.hip)
+// launchers (one translation unit per activation type: w4_f32.hip, w4_bf16.hip, w4_f16.hip, and w4_bf16_half.hip, w4_f16_half.hip
+// for rows that begin in the middle of a dword)
 // ---------------------------------------------------------------------------------------------
 hipError_t w4_launch_f32(const W4Params&, int scale_type, bool grad, hipStream_t);
 hipError_t w4_launch_bf16(const W4Params&, int scale_type, bool grad, hipStream_t);
 hipError_t w4_launch_f16(const W4Params&, int scale_type, bool grad, hipStream_t);
+hipError_t w4_launch_bf16_half(const W4Params&, int scale_type, bool grad, hipStream_t);      // rows that begin in the middle of a dword
+hipError_t w4_launch_f16_half(const W4Params&, int scale_type, bool grad, hipStream_t);
 
 #ifdef W4_KERNELS
-template <int DT, int ST, int NT, int MT, int GS, bool GRAD>
+template <int DT, int ST, bool HALF, int NT, int MT, int GS, bool GRAD>
 static hipError_t launch_rows(const W4Params& p, hipStream_t st) {
     constexpr int D = DT == GR_DT_F32 || NT > 1 || GRAD ? 1 : 2;
     const int64_t blocks = (int64_t)((p.R + 16 * MT - 1) / (16 * MT)) * ((p.N + 16 * NT - 1) / (16 * NT));
     int waves = blocks >= 2048 ? 4 : blocks >= 512 ? 8 : w4_rows_waves(NT);
     if (waves > p.chunks) waves = p.chunks;
     const size_t lds = (size_t)waves * MT * NT * 1024;
-    auto kern = &k_w4_rows<DT, ST, NT, MT, GS, D, GRAD>;
+    auto kern = &k_w4_rows<DT, ST, HALF, NT, MT, GS, D, GRAD>;
     if (lds > 64 * 1024) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return e;
@@ -894,24 +941,24 @@ static hipError_t launch_rows(const W4Params& p, hipStream_t st) {
     hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(waves * 64), lds, st, p);
     return hipGetLastError();
 }
-template <int DT, int ST, int NT, int MT, bool GRAD>
+template <int DT, int ST, bool HALF, int NT, int MT, bool GRAD>
 static hipError_t launch_rows(const W4Params& p, hipStream_t st) {
-    if constexpr (GRAD) return launch_rows<DT, ST, NT, MT, 1, true>(p, st);
-    else if (p.gsteps % 4 == 0) return launch_rows<DT, ST, NT, MT, 1, false>(p, st);
-    else if (p.gsteps % 2 == 0) return launch_rows<DT, ST, NT, MT, 2, false>(p, st);
-    else return launch_rows<DT, ST, NT, MT, 4, false>(p, st);
+    if constexpr (GRAD) return launch_rows<DT, ST, HALF, NT, MT, 1, true>(p, st);
+    else if (p.gsteps % 4 == 0) return launch_rows<DT, ST, HALF, NT, MT, 1, false>(p, st);
+    else if (p.gsteps % 2 == 0) return launch_rows<DT, ST, HALF, NT, MT, 2, false>(p, st);
+    else return launch_rows<DT, ST, HALF, NT, MT, 4, false>(p, st);
 }
-template <int DT, int ST, bool GRAD, int TM, int TN, int WM, int WN, int KS>
+template <int DT, int ST, bool HALF, bool GRAD, int TM, int TN, int WM, int WN, int KS>
 static hipError_t launch_gemm(const W4Params& p, hipStream_t st) {
     using G = W4Gemm<DT, GRAD, TM, TN, WM, WN, KS>;
-    auto kern = &k_w4_gemm<DT, ST, GRAD, TM, TN, WM, WN, KS>;
+    auto kern = &k_w4_gemm<DT, ST, HALF, GRAD, TM, TN, WM, WN, KS>;
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, G::LDS);
     if (e != hipSuccess) return e;
     const int64_t blocks = (int64_t)((p.R + G::BM - 1) / G::BM) * ((p.N + G::BN - 1) / G::BN);
     hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(G::NT), G::LDS, st, p);
     return hipGetLastError();
 }
-template <int DT, int ST, bool GRAD>
+template <int DT, int ST, bool HALF, bool GRAD>
 static hipError_t launch_typed(const W4Params& p, hipStream_t st) {
     // A variant's time is about that of one workgroup, which grows with the contraction, times the rounds that its workgroups
     // need:  max(1, workgroups / at_once) * (fixed + chunk * chunks)  microseconds, fitted to the variants' times at 1400 sizes (17
@@ -952,11 +999,11 @@ static hipError_t launch_typed(const W4Params& p, hipStream_t st) {
             consider(4, time(fwd[4], 64, 64, 1.f));
             consider(5, time(fwd[5], 128, tiled_cols, p.gsteps % 2 ? 1.3f : 1.f));     // groups of odd multiples of 32: more partial sums
         }
-        if (best == 0) return launch_rows<DT, ST, 1, 1, GRAD>(p, st);
-        if (best == 1) return launch_rows<DT, ST, 1, 2, GRAD>(p, st);
-        if (best == 2) return launch_rows<DT, ST, 2, 2, GRAD>(p, st);
-        if (best == 3) return launch_rows<DT, ST, 2, 4, GRAD>(p, st);
-        if (best == 4) return launch_rows<DT, ST, 4, 4, GRAD>(p, st);
+        if (best == 0) return launch_rows<DT, ST, HALF, 1, 1, GRAD>(p, st);
+        if (best == 1) return launch_rows<DT, ST, HALF, 1, 2, GRAD>(p, st);
+        if (best == 2) return launch_rows<DT, ST, HALF, 2, 2, GRAD>(p, st);
+        if (best == 3) return launch_rows<DT, ST, HALF, 2, 4, GRAD>(p, st);
+        if (best == 4) return launch_rows<DT, ST, HALF, 4, 4, GRAD>(p, st);
     } else {
         // a workgroup's row tiles share one group: its scales go to the activations
         const int most = p.gsteps % 4 == 0 ? 8 : p.gsteps % 2 == 0 ? 4 : 2;
@@ -967,19 +1014,19 @@ static hipError_t launch_typed(const W4Params& p, hipStream_t st) {
             if (most == 8) consider(3, time(grad[3], 128, 32, 1.f));
             consider(4, time(grad[4], 128, tiled_cols, 1.f));
         }
-        if (best == 0) return launch_rows<DT, ST, 1, 2, GRAD>(p, st);
-        if (best == 1) return launch_rows<DT, ST, 1, 4, GRAD>(p, st);
-        if (best == 2) return launch_rows<DT, ST, 2, 4, GRAD>(p, st);
-        if (best == 3) return launch_rows<DT, ST, 2, 8, GRAD>(p, st);
+        if (best == 0) return launch_rows<DT, ST, HALF, 1, 2, GRAD>(p, st);
+        if (best == 1) return launch_rows<DT, ST, HALF, 1, 4, GRAD>(p, st);
+        if (best == 2) return launch_rows<DT, ST, HALF, 2, 4, GRAD>(p, st);
+        if (best == 3) return launch_rows<DT, ST, HALF, 2, 8, GRAD>(p, st);
     }
-    if constexpr (DT == GR_DT_F32 || (GRAD && DT == GR_DT_F16)) return launch_gemm<DT, ST, GRAD, 4, 2, 2, 4, 1>(p, st);
-    else if constexpr (GRAD) return launch_gemm<DT, ST, GRAD, 4, 4, 2, 4, 1>(p, st);
-    else return launch_gemm<DT, ST, GRAD, 4, 4, 2, 4, 2>(p, st);
+    if constexpr (DT == GR_DT_F32 || (GRAD && DT == GR_DT_F16)) return launch_gemm<DT, ST, HALF, GRAD, 4, 2, 2, 4, 1>(p, st);
+    else if constexpr (GRAD) return launch_gemm<DT, ST, HALF, GRAD, 4, 4, 2, 4, 1>(p, st);
+    else return launch_gemm<DT, ST, HALF, GRAD, 4, 4, 2, 4, 2>(p, st);
 }
-template <int DT>
+template <int DT, bool HALF>
 static hipError_t launch_any(const W4Params& p, int scale_type, bool grad, hipStream_t st) {
-    if (scale_type == GR_DT_F32) return grad ? launch_typed<DT, GR_DT_F32, true>(p, st) : launch_typed<DT, GR_DT_F32, false>(p, st);
-    if (scale_type == GR_DT_BF16) return grad ? launch_typed<DT, GR_DT_BF16, true>(p, st) : launch_typed<DT, GR_DT_BF16, false>(p, st);
-    return grad ? launch_typed<DT, GR_DT_F16, true>(p, st) : launch_typed<DT, GR_DT_F16, false>(p, st);
+    if (scale_type == GR_DT_F32) return grad ? launch_typed<DT, GR_DT_F32, HALF, true>(p, st) : launch_typed<DT, GR_DT_F32, HALF, false>(p, st);
+    if (scale_type == GR_DT_BF16) return grad ? launch_typed<DT, GR_DT_BF16, HALF, true>(p, st) : launch_typed<DT, GR_DT_BF16, HALF, false>(p, st);
+    return grad ? launch_typed<DT, GR_DT_F16, HALF, true>(p, st) : launch_typed<DT, GR_DT_F16, HALF, false>(p, st);
 }
 #endif

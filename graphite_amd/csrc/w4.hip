@@ -119,8 +119,9 @@ extern "C" int gr_w4_create(gr_ctx* ctx, const uint8_t* q, int64_t ldq, const vo
 
 static hipError_t w4_launch(const W4Params& p, int dt, int scale_type, bool grad, hipStream_t st) {
     if (dt == GR_DT_F32) return w4_launch_f32(p, scale_type, grad, st);
-    if (dt == GR_DT_BF16) return w4_launch_bf16(p, scale_type, grad, st);
-    return w4_launch_f16(p, scale_type, grad, st);
+    const bool half = (uintptr_t)p.x % 4 || (p.N > 1 && p.ldx % 2);       // some row begins in the middle of a dword
+    if (dt == GR_DT_BF16) return half ? w4_launch_bf16_half(p, scale_type, grad, st) : w4_launch_bf16(p, scale_type, grad, st);
+    return half ? w4_launch_f16_half(p, scale_type, grad, st) : w4_launch_f16(p, scale_type, grad, st);
 }
 
 static int w4_run(gr_ctx* ctx, const gr_w4* w, const char* who, bool grad, const void* x, int dt, int64_t N, int64_t ldx, const void* gate,

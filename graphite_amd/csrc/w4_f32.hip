@@ -3,5 +3,5 @@
 #include "w4.h"
 
 hipError_t w4_launch_f32(const W4Params& p, int scale_type, bool grad, hipStream_t st) {
-    return launch_any<GR_DT_F32>(p, scale_type, grad, st);
+    return launch_any<GR_DT_F32, false>(p, scale_type, grad, st);
 }

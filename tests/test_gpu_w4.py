@@ -327,3 +327,28 @@ def test_c_entry_refusals():
     for bad in (dict(w=None), dict(x=None), dict(y=None), dict(dt=3), dict(n=-1), dict(ldx=63), dict(ldy=15), dict(n=2 ** 40)):
         assert f(**bad) == -1 and lib.gr_last_error(ctx)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("n,length", [(1, 5), (1, 75), (3, 7), (17, 131), (40, 8), (64, 255), (150, 401), (700, 333), (2600, 521)])
+def test_rows_that_begin_inside_a_dword(dtype, n, length):
+    """Where a row begins in memory must not change a bit of its result, nor must what lies beside it: the sums and their order
+    are those of aligned rows, so equality is exact."""
+    g = torch.Generator().manual_seed(n + length)
+    other = 300
+    for grad in (False, True):
+        m, k = (length, other) if grad else (other, length)
+        w = (torch.randn(m, k, generator=g) / length ** 0.5).cuda()
+        group = 128 if k >= 128 else 32
+        q, s, z = (v.cuda() for v in quantize(w, group))
+        layer = LinearW4(q, s, z, group=group, in_features=k, input_grad=grad)
+        x = torch.randn(n, length, generator=g).cuda().to(dtype)
+        run = layer.input_grad if grad else layer.forward
+        even = torch.zeros(n, length + length % 2, device="cuda", dtype=dtype)[:, :length]
+        even.copy_(x)
+        expect = run(even)
+        for first, gap in ((0, 1 - length % 2), (1, 0), (1, 1), (3, 8), (2, 5)):
+            flat = torch.full((first + n * (length + gap) + 1,), float("nan"), device="cuda", dtype=dtype)
+            rows = torch.as_strided(flat, (n, length), (length + gap, 1), first)
+            rows.copy_(x)
+            assert torch.equal(run(rows), expect), (grad, first, gap)
