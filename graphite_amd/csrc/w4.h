@@ -859,16 +859,20 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
             read_qa(b0, 0);
 #pragma unroll
             for (int t = 0; t < TN; t++) read_qx(0, b0, t);
-            if (p.gsteps % 2)
-                for (; s + 2 <= plain; s += 2) {
-                    body16.template operator()<true, 0>(s);
-                    body16.template operator()<true, 1>(s + 1);
-                }
-            else
+            bool perstep = false;
+            if constexpr (TN == 2) perstep = p.gsteps % 2;             // the whole tile is not used for such groups
+            if (perstep) {
+                if constexpr (TN == 2)
+                    for (; s + 2 <= plain; s += 2) {
+                        body16.template operator()<true, 0>(s);
+                        body16.template operator()<true, 1>(s + 1);
+                    }
+            } else {
                 for (; s + 2 <= plain; s += 2) {
                     body16.template operator()<false, 0>(s);
                     body16.template operator()<false, 1>(s + 1);
                 }
+            }
             crem = s * KS % p.gsteps;
         }
     } else if (plain >= 2 && (GRAD || p.gsteps % 2 == 0)) {
@@ -960,30 +964,38 @@ static hipError_t launch_gemm(const W4Params& p, hipStream_t st) {
 }
 template <int DT, int ST, bool HALF, bool GRAD>
 static hipError_t launch_typed(const W4Params& p, hipStream_t st) {
-    // A variant's time is about that of one workgroup, which grows with the contraction, times the rounds that its workgroups
-    // need:  max(1, workgroups / at_once) * (fixed + chunk * chunks)  microseconds, fitted to the variants' times at 1400 sizes (17
-    // to 8192 rows, 33 to 8192 on both sides, every group).  The variant with the least estimate takes 3 to 5 % longer than the
-    // fastest one (geometric mean); limits on the number of output tiles took 5 to 9 % and up to 2.3 times as long.
+    // A variant's time is about that of a workgroup, which grows with the contraction, times the rounds that its workgroups need,
+    // and something for each output.  In microseconds:  out * workgroups / 256 + chunk * chunks * rounds, where rounds is
+    //   max(1, workgroups / (256 * more))            for small workgroups, several of which share a CU,
+    //   1 + more * (ceil(workgroups / 256) - 1)      for large ones (LDS), one a CU.
+    // The numbers are fitted to the variants' times at 900 sizes (17 to 8192 rows, 33 to 8192 on both sides, every group).  The
+    // variant with the least estimate takes 3 to 6 % longer than the fastest one (geometric mean); limits on the number of
+    // output tiles took 6 to 13 % and up to 3.3 times as long.
     // Small tiles carry short contractions and few rows, the tiled kernel large products (us, in the order of `fwd`):  bf16,
     // 320 rows 96 -> 6528  10.7 8.4 9.3 10.3 14.4 11.5;  f32, 384 rows 7680 -> 2848  -, -, 169 122 217 184;  bf16, 2464 rows
-    // 3648 -> 2048  -, -, 159 110 138 81.
-    struct Cost { float fixed, chunk, at_once; };
+    // 3648 -> 2048  -, -, 159 110 138 81.  The tiled kernel's half tile: 2048 rows 4096 -> 4096 bf16, groups of 128  116 (whole
+    // 95), of 32  118 (130: twice the partial sums, and registers spilled).
+    struct Cost { float out, chunk, more; };
     constexpr bool F32 = DT == GR_DT_F32, F16 = DT == GR_DT_F16;
-    constexpr Cost fwd[6] = {F32 ? Cost{0.05f, 0.18f, 197.f} : Cost{0.05f, 0.09f, 184.f},      // row tiles x batch tiles: 1 x 1
-                             F32 ? Cost{0.05f, 0.22f, 180.f} : Cost{0.05f, 0.11f, 151.f},      // 2 x 1
-                             F32 ? Cost{0.11f, 0.46f, 172.f} : Cost{0.15f, 0.23f, 184.f},      // 2 x 2
-                             F32 ? Cost{0.36f, 0.59f, 154.f} : Cost{0.33f, 0.35f, 169.f},      // 4 x 2
-                             F32 ? Cost{3.82f, 1.68f, 223.f} : Cost{3.77f, 0.57f, 218.f},      // 4 x 4
-                             F32 ? Cost{0.05f, 2.87f, 154.f} : Cost{0.79f, 2.87f, 125.f}};     // tiled
-    constexpr Cost grad[5] = {F32 ? Cost{0.05f, 0.29f, 182.f} : Cost{0.05f, 0.21f, 176.f},     // 2 x 1
-                              F32 ? Cost{0.06f, 0.34f, 184.f} : Cost{0.05f, 0.29f, 183.f},     // 4 x 1
-                              F32 ? Cost{0.16f, 0.70f, 172.f} : Cost{0.28f, 0.55f, 183.f},     // 4 x 2
-                              F32 ? Cost{1.42f, 1.00f, 200.f} : Cost{1.86f, 0.78f, 218.f},     // 8 x 2
-                              F32 ? Cost{0.05f, 4.16f, 143.f} : F16 ? Cost{0.05f, 3.02f, 148.f} : Cost{0.05f, 3.24f, 118.f}};  // tiled
-    auto time = [&](const Cost& c, int rows, int cols, float slower) {          // of workgroups of rows x cols outputs
-        const float blocks = (float)((p.R + rows - 1) / rows) * (float)((p.N + cols - 1) / cols);
-        return (blocks > c.at_once ? blocks / c.at_once : 1.f) * (c.fixed + c.chunk * slower * (float)p.chunks);
+    constexpr Cost fwd[7] = {F32 ? Cost{0.05f, 0.16f, 0.67f} : Cost{0.05f, 0.09f, 0.83f},      // row tiles x batch tiles: 1 x 1
+                             F32 ? Cost{0.05f, 0.22f, 0.71f} : Cost{0.05f, 0.11f, 0.68f},      // 2 x 1
+                             F32 ? Cost{0.05f, 0.47f, 0.69f} : Cost{0.09f, 0.21f, 0.74f},      // 2 x 2
+                             F32 ? Cost{0.30f, 0.59f, 0.60f} : Cost{0.18f, 0.31f, 0.57f},      // 4 x 2
+                             F32 ? Cost{2.64f, 2.69f, 0.75f} : Cost{2.32f, 0.58f, 1.25f},      // 4 x 4
+                             F32 ? Cost{2.88f, 2.80f, 1.32f} : Cost{5.72f, 2.91f, 1.20f},      // tiled
+                             Cost{2.67f, 1.39f, 1.50f}};                                       // tiled, half the batch rows (16-bit)
+    constexpr Cost grad[5] = {F32 ? Cost{0.05f, 0.28f, 0.72f} : Cost{0.05f, 0.20f, 0.77f},     // 2 x 1
+                              F32 ? Cost{0.05f, 0.34f, 0.70f} : Cost{0.05f, 0.28f, 0.72f},     // 4 x 1
+                              F32 ? Cost{0.06f, 0.67f, 0.61f} : Cost{0.15f, 0.49f, 0.63f},     // 4 x 2
+                              F32 ? Cost{0.80f, 1.08f, 1.26f} : Cost{1.35f, 0.78f, 1.15f},     // 8 x 2
+                              F32 ? Cost{2.19f, 3.97f, 1.72f} : F16 ? Cost{0.69f, 2.76f, 1.82f} : Cost{4.08f, 3.20f, 1.43f}};  // tiled
+    auto time = [&](const Cost& c, int rows, int cols, bool large, float slower) {          // of workgroups of rows x cols outputs
+        const int64_t blocks = (int64_t)((p.R + rows - 1) / rows) * ((p.N + cols - 1) / cols);
+        const float share = (float)blocks / 256.f;
+        const float rounds = large ? 1.f + c.more * (float)((blocks + 255) / 256 - 1) : share > c.more ? share / c.more : 1.f;
+        return c.out * share + c.chunk * slower * (float)p.chunks * rounds;
     };
+    const bool odd = p.gsteps % 2;                         // groups end inside 64 steps: the tiled kernels' partial sums end every 32
     constexpr int tiled_cols = F32 || (GRAD && F16) ? 128 : 256;
     int best = 0;
     float least = 3e38f;
@@ -991,13 +1003,14 @@ static hipError_t launch_typed(const W4Params& p, hipStream_t st) {
         if (t < least) { least = t; best = i; }
     };
     if constexpr (!GRAD) {
-        consider(0, time(fwd[0], 16, 16, 1.f));
-        consider(1, time(fwd[1], 32, 16, 1.f));
+        consider(0, time(fwd[0], 16, 16, false, 1.f));
+        consider(1, time(fwd[1], 32, 16, false, 1.f));
         if (p.N > 16) {
-            consider(2, time(fwd[2], 32, 32, 1.f));
-            consider(3, time(fwd[3], 64, 32, 1.f));
-            consider(4, time(fwd[4], 64, 64, 1.f));
-            consider(5, time(fwd[5], 128, tiled_cols, p.gsteps % 2 ? 1.3f : 1.f));     // groups of odd multiples of 32: more partial sums
+            consider(2, time(fwd[2], 32, 32, false, 1.f));
+            consider(3, time(fwd[3], 64, 32, false, 1.f));
+            consider(4, time(fwd[4], 64, 64, true, 1.f));
+            if (F32 || !odd) consider(5, time(fwd[5], 128, tiled_cols, true, odd ? 1.2f : 1.f));
+            if (!F32) consider(6, time(fwd[6], 128, 128, true, odd ? 1.1f : 1.f));
         }
         if (best == 0) return launch_rows<DT, ST, HALF, 1, 1, GRAD>(p, st);
         if (best == 1) return launch_rows<DT, ST, HALF, 1, 2, GRAD>(p, st);
@@ -1007,12 +1020,12 @@ static hipError_t launch_typed(const W4Params& p, hipStream_t st) {
     } else {
         // a workgroup's row tiles share one group: its scales go to the activations
         const int most = p.gsteps % 4 == 0 ? 8 : p.gsteps % 2 == 0 ? 4 : 2;
-        consider(0, time(grad[0], 32, 16, 1.f));
-        if (most >= 4) consider(1, time(grad[1], 64, 16, 1.f));
+        consider(0, time(grad[0], 32, 16, false, 1.f));
+        if (most >= 4) consider(1, time(grad[1], 64, 16, false, 1.f));
         if (p.N > 16) {
-            if (most >= 4) consider(2, time(grad[2], 64, 32, 1.f));
-            if (most == 8) consider(3, time(grad[3], 128, 32, 1.f));
-            consider(4, time(grad[4], 128, tiled_cols, 1.f));
+            if (most >= 4) consider(2, time(grad[2], 64, 32, false, 1.f));
+            if (most == 8) consider(3, time(grad[3], 128, 32, true, 1.f));
+            consider(4, time(grad[4], 128, tiled_cols, true, 1.f));
         }
         if (best == 0) return launch_rows<DT, ST, HALF, 1, 2, GRAD>(p, st);
         if (best == 1) return launch_rows<DT, ST, HALF, 1, 4, GRAD>(p, st);
@@ -1021,6 +1034,7 @@ static hipError_t launch_typed(const W4Params& p, hipStream_t st) {
     }
     if constexpr (DT == GR_DT_F32 || (GRAD && DT == GR_DT_F16)) return launch_gemm<DT, ST, HALF, GRAD, 4, 2, 2, 4, 1>(p, st);
     else if constexpr (GRAD) return launch_gemm<DT, ST, HALF, GRAD, 4, 4, 2, 4, 1>(p, st);
+    else if (best == 6) return launch_gemm<DT, ST, HALF, GRAD, 4, 2, 2, 4, 2>(p, st);
     else return launch_gemm<DT, ST, HALF, GRAD, 4, 4, 2, 4, 2>(p, st);
 }
 template <int DT, bool HALF>
