@@ -1008,7 +1008,8 @@ static hipError_t launch_typed(const W4Params& p, hipStream_t st) {
         if (p.N > 16) {
             consider(2, time(fwd[2], 32, 32, false, 1.f));
             consider(3, time(fwd[3], 64, 32, false, 1.f));
-            consider(4, time(fwd[4], 64, 64, true, 1.f));
+            // 4 x 4 spills registers where a chunk has several groups or rows begin inside a dword: measured against the above
+            consider(4, time(fwd[4], 64, 64, true, (odd ? 1.4f : p.gsteps % 4 ? 1.1f : 1.f) * (HALF ? 1.5f : 1.f)));
             if (F32 || !odd) consider(5, time(fwd[5], 128, tiled_cols, true, odd ? 1.2f : 1.f));
             if (!F32) consider(6, time(fwd[6], 128, 128, true, odd ? 1.1f : 1.f));
         }
