@@ -932,7 +932,7 @@ hipError_t w4_launch_f16_half(const W4Params&, int scale_type, bool grad, hipStr
 #ifdef W4_KERNELS
 template <int DT, int ST, bool HALF, int NT, int MT, int GS, bool GRAD>
 static hipError_t launch_rows(const W4Params& p, hipStream_t st) {
-    constexpr int D = DT == GR_DT_F32 || NT > 1 || GRAD ? 1 : 2;
+    constexpr int D = DT == GR_DT_F32 || NT > 1 || GRAD || HALF ? 1 : 2;
     const int64_t blocks = (int64_t)((p.R + 16 * MT - 1) / (16 * MT)) * ((p.N + 16 * NT - 1) / (16 * NT));
     int waves = blocks >= 2048 ? 4 : blocks >= 512 ? 8 : w4_rows_waves(NT);
     if (waves > p.chunks) waves = p.chunks;
