@@ -271,7 +271,7 @@ __device__ __forceinline__ void w4_put(const W4Params& p, w4_f32x4 sum, const fl
 // axis is split inside the workgroup, so there is no workspace, no second launch and one order of summation.
 // Forward: GS = groups of a chunk (1, 2 or 4; 4 also where a border falls on any step).
 // One row is bound by the weights' bytes: the matrix unit pads it to 16 rows for nothing, and what costs is turning nibbles
-// into operands, 2.5 VALU instructions a weight.  8192 -> 8192 bf16, g = 128, one row: 10.4 us = 3.4 TB/s of weights (a copy
+// into operands, 2.5 VALU instructions a weight.  8192 -> 8192 bf16, g = 128, one row: 10.8 us = 3.2 TB/s of weights (a copy
 // reaches 4.7).  2048 -> 1024 f32, 100 rows: 8.1 us a call (its latency: two chunks a wave, then the join, in which a thread
 // adds and stores four outputs at once; one output a thread took 9.2).
 // ---------------------------------------------------------------------------------------------
@@ -467,12 +467,13 @@ __global__ __launch_bounds__(w4_rows_waves(NT) * 64) void k_w4_rows(W4Params p) 
 // [16 bytes], the order the packed weights already have), so every LDS access is 64 lanes x 16 consecutive bytes.
 // Three LDS buffers, one barrier per stage: while a stage is multiplied, the next one's first operands are already read and
 // the one after is written, from registers that global memory filled a stage earlier.
-// Measured (4096 -> 4096, 4096 rows, bf16): 192 us = 715 TFLOP/s, a library product of that size 1220; its gradient at 2048 rows
-// 130 us = 530 (1060 of matrix work, two pieces); 8192 x 2048 -> 1024 f32 126 us = 272 (816 of matrix work; the f32 matrix
-// unit's peak is 157).  Nothing is saturated: the matrix unit is busy 29 % of the cycles (gradient 40), VALU issue takes 41,
-// LDS 29; two waves a SIMD, in step through the barrier, overlap them only in part.  Tried and slower: 4-wave workgroups of
-// 128 x 128 (251 us), halves of the waves taking turns at multiplying and staging (570 us), loads two stages ahead (no gain),
-// partial sums held over whole groups (219 us: 64 registers spilled), raised wave priority (+10 %).
+// Measured (4096 -> 4096, 4096 rows, bf16): 160 us = 857 TFLOP/s, a library product of that size 1220; its gradient at 2048 rows
+// 131 us = 525 (1050 of matrix work, two pieces); 8192 x 2048 -> 1024 f32 118 us = 291 (873 of matrix work; the f32 matrix
+// unit's peak is 157).  Nothing is saturated: the matrix unit is busy 35 % of the cycles (gradient 40), VALU issue takes 46,
+// LDS 35; two waves a SIMD, in step through the barrier, overlap them only in part.  Tried and slower, against 192 us at the
+// time (the code for groups of 32 still in the same kernel, which spilled for it):  4-wave workgroups of 128 x 128 (251 us),
+// halves of the waves taking turns at multiplying and staging (570 us), loads two stages ahead (no gain), partial sums held
+// over whole groups (219 us: 64 registers spilled), raised wave priority (+10 %).
 // ---------------------------------------------------------------------------------------------
 template <int DT, bool GRAD> struct W4Pieces {          // pieces of the weights and of the activations
     static constexpr int W = !GRAD ? 1 : DT == GR_DT_F32 ? 3 : 2;
@@ -991,6 +992,7 @@ static hipError_t launch_typed(const W4Params& p, hipStream_t st) {
                               F32 ? Cost{2.19f, 3.97f, 1.72f} : F16 ? Cost{0.69f, 2.76f, 1.82f} : Cost{4.08f, 3.20f, 1.43f}};  // tiled
     auto time = [&](const Cost& c, int rows, int cols, bool large, float slower) {          // of workgroups of rows x cols outputs
         const int64_t blocks = (int64_t)((p.R + rows - 1) / rows) * ((p.N + cols - 1) / cols);
+        if (rows * cols < 128 * 128 && blocks > 1 << 23) return 1e30f;      // threads of a launch are counted in 32 bits
         const float share = (float)blocks / 256.f;
         const float rounds = large ? 1.f + c.more * (float)((blocks + 255) / 256 - 1) : share > c.more ? share / c.more : 1.f;
         return c.out * share + c.chunk * slower * (float)p.chunks * rounds;

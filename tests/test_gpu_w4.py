@@ -352,3 +352,32 @@ def test_rows_that_begin_inside_a_dword(dtype, n, length):
             rows = torch.as_strided(flat, (n, length), (length + gap, 1), first)
             rows.copy_(x)
             assert torch.equal(run(rows), expect), (grad, first, gap)
+
+
+def test_rows_past_32_bits():
+    """More than 2^32 elements, and more small tiles than a launch holds: every offset and the choice of the kernel."""
+    n, k, m = 140_000_003, 33, 10
+    layer, w, _ = _layer(m, k, 32, sdt=F16)
+    with_grad = LinearW4(*_packed(m, k), group=32, in_features=k, input_grad=True)
+    rows = torch.tensor([0, 1, 65_075_262, 65_075_263, 130_150_524, 130_150_525, n - 2, n - 1], device="cuda")
+    for run, a, b, ref in ((layer.forward, k, m, w.T), (with_grad.input_grad, m, k, w)):
+        x = torch.zeros(n, a, device="cuda", dtype=F16)
+        vals = torch.randn(len(rows), a, generator=torch.Generator().manual_seed(3)).to(F16)
+        x[rows] = vals.cuda()
+        y = run(x)
+        del x
+        v = vals.double().numpy()
+        expect, mag = v @ ref, np.abs(v) @ np.abs(ref)
+        assert (np.abs(y[rows].cpu().double().numpy() - expect) <= _tol(expect, mag, a, F16, 2.0 ** -15)).all()
+        y[rows] = 0
+        assert not y.any()
+        del y
+    torch.cuda.empty_cache()
+
+
+def _packed(m, k):
+    g = torch.Generator().manual_seed(0)                                            # the tensors of _layer(m, k, 32, F16)
+    q = torch.randint(0, 256, (m, (k + 1) // 2), generator=g, dtype=torch.uint8)
+    groups = -(-k // 32)
+    s = (torch.rand((m, groups), generator=g) * 0.02 + 0.001).to(F16)
+    return q.cuda(), s.cuda(), torch.randint(0, 16, (m, groups), generator=g, dtype=torch.uint8).cuda()
