@@ -4,7 +4,9 @@
 //   mr = max z_i,  w_i = exp2((z_i - mr) c),  Sr = sum w_i                                   one pass, running maximum and sum
 //   M = max(mr, max of the named z),  St = Sr exp2((mr - M) c) + sum over named of exp2((z_j - M) c)
 // the student's log-probabilities are  log q_j = (z_j - M) c ln2 - ln St  and  log q_rest = ln Sr + (mr - M) c ln2 - ln St, and
-//   d loss / d z_i = tau (w_i exp2((mr - M) c) / St - p_rest w_i / Sr)   unnamed,   tau (q_j - p_j)   named.
+//   d loss / d z_i = tau (P q_i - p_rest w_i / Sr),  q_i = w_i exp2((mr - M) c) / St   unnamed,   tau (P q_j - p_j)   named,
+// P = what the loss's terms hold of the teacher: 1, but the sum of the named p_j where no p_rest enters (it is 0, p_j of rounded
+// logits adding up to 1 or more, or no unnamed class can take it): the softmax's normaliser then has that much weight.
 // The unnamed sum has its own maximum, so q_rest keeps its digits when the named classes hold nearly everything (a difference
 // 1 - sum q_j would not).  The teacher's few values are handled in 64 bits: p_rest IS a difference, next to zero.
 #include "common.h"
@@ -321,10 +323,11 @@ __global__ __launch_bounds__(NT) void k_distill(KdParams p) {
     const float St = part + Sr * shift;
     const bool tail = OPEN && !(rest <= 0.) && !(none && Sr == 0.f);
     const float a0 = gl * p.tau;
+    const float P = OPEN && !tail ? (float)mass : 1.f;
     // Unnamed gradients are a0 w_i / Sr (q_rest - p_rest): where the two are near 1, their difference is taken from what the
     // named classes hold on either side, else directly.
     const float q_rest = Sr * shift / St;
-    const float A = !tail ? a0 * (shift / St) : a0 / Sr * (rest > 0.5 ? (float)mass - part / St : q_rest - (float)rest);
+    const float A = !tail ? a0 * P * (shift / St) : a0 / Sr * (rest > 0.5 ? (float)mass - part / St : q_rest - (float)rest);
     if (g) {
         const bool same = (uintptr_t)(g + h) % 16 == 0;
         kd_u32x4* gv = (kd_u32x4*)(g + h);
@@ -367,7 +370,7 @@ __global__ __launch_bounds__(NT) void k_distill(KdParams p) {
         pj *= inv;
         const float d = ex.arg(s_z[j], M);
         if (pj > 0. || pj != pj) kl += pj * (log(pj) - (((double)s_z[j] - (double)M) * p.inv_tau - lnS));
-        if (g) g[ij] = (T)(a0 * (__builtin_amdgcn_exp2f(d) / St - (float)pj));
+        if (g) g[ij] = (T)(a0 * (P * (__builtin_amdgcn_exp2f(d) / St) - (float)pj));
     }
     if (p.loss) {
         kl = kd_wave(kl, 0., add);

@@ -316,7 +316,8 @@ int gr_linear_w4_input_grad(gr_ctx* ctx, const gr_w4* w, const void* grad_y, int
  *                                 class with q_rest = the student's mass outside the named classes (nothing if that set is
  *                                 empty or all its logits are -inf)
  *   loss[n] = tau^2 * ( sum_j p_j log(p_j / q_j) + p_rest log(p_rest / q_rest) )                     float32, or NULL
- *   grad[n,:] = grad_loss[n] * d loss[n] / d z[n,:]  (type dtype, rows ldg apart; NULL = not wanted; grad_loss NULL = 1)
+ *   grad[n,:] = grad_loss[n] * d loss[n] / d z[n,:]  (type dtype, rows ldg apart; NULL = not wanted; grad_loss NULL = 1):
+ *               tau (P q_i - target_i) with P = sum p + p_rest, p_rest counted only where the loss counts it
  * grad may be z itself (ldg == ldz) but must not overlap it otherwise.  A row without slots (all -1; closed: also all values -inf) has loss 0 and gradient 0.
  * An index outside [-1, V) makes its row's loss and gradient NaN.  1 <= k <= 1024; 1e-6 <= tau <= 1e6; V <= 2^20 in the
  * open form.  No workspace, no allocation: the call can be captured into a HIP graph.  Results do not vary between runs. */

@@ -63,14 +63,14 @@ def distill_row(z, index, value, tau, lse=None):
     named[idx] = True
     terms = p[named] > 0
     loss = float((p[named][terms] * (np.log(p[named][terms]) - log_q[named][terms])).sum())
-    target = p
+    target = p                                     # loss = constant - sum_i target_i log q_i: gradient sum(target) q - target
     if lse is not None:
         rest = max(0.0, 1.0 - float(np.exp(t - float(lse)).sum()))
         log_qr = _lse(log_q[~named])
         if rest > 0 and np.isfinite(log_qr):
             loss += rest * (math.log(rest) - log_qr)
             target = p + np.where(named, 0.0, rest * np.exp(log_q - log_qr))
-    return tau * tau * loss, tau * (np.exp(log_q) - target)
+    return tau * tau * loss, tau * (target.sum() * np.exp(log_q) - target)
 
 
 def distill(z, index, value, tau, lse=None, grad_loss=None):

@@ -245,3 +245,41 @@ def test_refusals():
     assert abs(float(loss) - np.log(2 ** 20 + 1)) <= 1e-4 and abs(float(grad[0, 7]) + 1) <= 1e-5
     loss, grad = topk_distill(wide[:, 1:], i, v, teacher_lse=torch.full((1,), np.log(2.0), device="cuda"))
     assert abs(float(loss) - (0.5 * np.log(0.5 * 2 ** 20) + 0.5 * np.log(0.5))) <= 1e-4
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("v", [43, 3000, 40001])
+@pytest.mark.parametrize("case", ["nothing_unnamed_is_left", "named_mass_above_one"])
+def test_gradient_where_the_target_does_not_add_up_to_one(case, v, dtype):
+    """No p_rest enters the loss: every unnamed student logit is -inf, or the named p_j (of logits rounded to bfloat16, beside
+    the float32 logsumexp of the unrounded ones) add up to more than 1.  Against the 64-bit gradient, and against central
+    differences of the 64-bit loss: step 2^-10, their own error h^2 / 6 times the third derivative, at most 2 P, P < 2."""
+    g = torch.Generator().manual_seed(27)
+    n, k, tau = 3, 4, 1.0
+    z = (torch.randn((n, v), generator=g) * 2.5).cuda()
+    t = (torch.randn((n, v), generator=g) * 1.5).cuda()
+    if case == "named_mass_above_one":
+        hot = torch.tensor([[25.07, 25.19, 24.06, 23.07]], device="cuda")     # each goes up when rounded to bfloat16
+        t[:, 5:9] = hot
+    top = teacher_top(t, k, tau)
+    value = top.value.to(BF16) if case == "named_mass_above_one" else top.value
+    if case == "nothing_unnamed_is_left":
+        named = torch.zeros((n, v), dtype=torch.bool, device="cuda").scatter_(1, top.index, True)
+        z = torch.where(named, z, torch.full_like(z, float("-inf")))
+    z = z.to(dtype)
+    mass = torch.exp(value.double() / tau - top.lse.double()[:, None]).sum(1)
+    assert bool((mass > 1.02).all()) if case == "named_mass_above_one" else bool((mass < 0.98).all())
+    gl = torch.rand(n, generator=g).cuda() + 0.1
+    loss, grad = topk_distill(z, top.index, value, tau, top.lse, gl)
+    _compare(z, top.index, value, tau, top.lse, gl, loss, grad)
+    zd, h = z.double().cpu().numpy(), 2.0 ** -10
+    a = (top.index.cpu().numpy(), value.double().cpu().numpy(), tau, top.lse.double().cpu().numpy(), gl.double().cpu().numpy())
+    gd = grad.double().cpu().numpy()
+    scale = gl.double().cpu().numpy()
+    for i in [int(top.index[0, 0]), int(top.index[0, 3])] + ([0, 9] if case == "named_mass_above_one" else []):
+        d = np.zeros_like(zd)
+        d[:, i] = h
+        up, down = R.distill(zd + d, *a)[0], R.distill(zd - d, *a)[0]
+        fd = np.where(np.isfinite(zd[:, i]), scale * (up - down) / (2 * h), 0.0)
+        tol = scale * 2 * (1e-6 + 4 * 1100 * 2.0 ** -24) + np.abs(gd[:, i]) * torch.finfo(dtype).eps / 2
+        assert (np.abs(gd[:, i] - fd) <= tol).all()

@@ -88,3 +88,30 @@ def test_reference_gradient_is_the_difference_of_its_losses(rest):
         fd = (R.distill(z + d, idx, val, 1.5, lse)[0] - R.distill(z - d, idx, val, 1.5, lse)[0]) / 2e-5
         assert np.abs(fd - grad[:, i]).max() <= 1e-8
     assert (loss > 0).all() and np.abs(grad.sum(1)).max() <= 1e-12
+
+
+@pytest.mark.parametrize("case", ["nothing_unnamed_is_left", "named_mass_above_one", "all_classes_named"])
+def test_reference_gradient_where_the_target_does_not_add_up_to_one(case):
+    """Open form without a p_rest term: the named p_j alone weigh the loss, and the softmax's normaliser takes their sum."""
+    g = np.random.default_rng(2)
+    v = 10
+    z, t = g.standard_normal((2, v)) * 2, g.standard_normal((2, v)) * 2
+    k = v if case == "all_classes_named" else 4
+    idx = np.argsort(-t, 1)[:, :k]
+    val = np.take_along_axis(t, idx, 1)
+    lse = np.log(np.exp(t / 1.5).sum(1))
+    if case == "nothing_unnamed_is_left":
+        keep = np.take_along_axis(z, idx, 1)
+        z[:] = -np.inf
+        np.put_along_axis(z, idx, keep, 1)
+    else:
+        lse = lse - (0.8 if case == "named_mass_above_one" else -0.3)
+    mass = np.exp(val / 1.5 - lse[:, None]).sum(1)
+    assert (mass > 1.05).all() if case == "named_mass_above_one" else (mass < 0.95).all()
+    _, grad = R.distill(z, idx, val, 1.5, lse)
+    assert not grad[~np.isfinite(z)].any() and np.abs(grad.sum(1)).max() <= 1e-12
+    for i in range(v):
+        d = np.zeros_like(z)
+        d[:, i] = 1e-5
+        fd = (R.distill(z + d, idx, val, 1.5, lse)[0] - R.distill(z - d, idx, val, 1.5, lse)[0]) / 2e-5
+        assert np.abs(np.where(np.isfinite(z[:, i]), fd - grad[:, i], 0.0)).max() <= 1e-8
