@@ -6,7 +6,6 @@
 
 struct gr_w4 {
     gr_ctx* ctx = nullptr;
-    int device = 0;
     int M = 0, K = 0, group = 0, G = 0, st = 0, Mp = 0, Kp = 0;
     bool has_zeros = false;              // else `zeros` is one row of eights
     char* mem = nullptr;                 // one allocation: pack | transposed pack | scales | zeros | bias
@@ -57,10 +56,7 @@ int w4_in_features(const gr_w4* w) { return w->K; }
 
 extern "C" void gr_w4_destroy(gr_w4* w) {
     if (!w) return;
-    if (w->mem) {
-        (void)hipSetDevice(w->device);
-        (void)hipFree(w->mem);
-    }
+    if (w->mem) (void)hipFree(w->mem);       // the memory knows its device; the caller's current one stays
     delete w;
 }
 
@@ -81,7 +77,7 @@ extern "C" int gr_w4_create(gr_ctx* ctx, const uint8_t* q, int64_t ldq, const vo
     hipStream_t st = (hipStream_t)stream;
     gr_w4* w = new (std::nothrow) gr_w4();
     if (!w) return gr_fail(ctx, GR_ENOMEM, "gr_w4_create: out of host memory");
-    w->ctx = ctx; w->device = ctx->device; w->M = M; w->K = K; w->group = group; w->G = G; w->st = scale_type; w->has_zeros = zeros != nullptr;
+    w->ctx = ctx; w->M = M; w->K = K; w->group = group; w->G = G; w->st = scale_type; w->has_zeros = zeros != nullptr;
     w->Mp = (M + 127) / 128 * 128; w->Kp = (K + 127) / 128 * 128;
     const size_t pk = (size_t)w->Mp * w->Kp / 2, ssz = gr_align((size_t)G * w->Mp * dt_size(scale_type));
     const size_t zsz = gr_align((size_t)(zeros ? G : 1) * w->Mp), bsz = bias ? gr_align((size_t)M * 4) : 0;
