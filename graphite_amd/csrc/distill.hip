@@ -27,6 +27,7 @@ struct KdParams {
     const int64_t* index; const void* value; int vt;
     const float *lse, *grad_loss; float* loss;
     int64_t N, ldz, ldg, ld_top;
+    int64_t n0;              // first row of this launch
     int V, k;
     float tau;
     double inv_tau;
@@ -155,7 +156,7 @@ __global__ __launch_bounds__(NT) void k_distill(KdParams p) {
     float* s_z = (float*)(s_p + p.k);
     int* s_i = (int*)(s_z + p.k);
     unsigned* s_bits = (unsigned*)(s_i + p.k);
-    const int64_t n = blockIdx.x;
+    const int64_t n = p.n0 + blockIdx.x;
     const int tid = threadIdx.x, V = p.V, k = p.k;
     const T* z = (const T*)p.z + n * p.ldz;
     T* g = p.grad ? (T*)p.grad + n * p.ldg : nullptr;
@@ -381,15 +382,21 @@ __global__ __launch_bounds__(NT) void k_distill(KdParams p) {
 }
 
 template <int DT, int NT, int VPT, bool BIG, bool OPEN>
-hipError_t launch1(const KdParams& p, hipStream_t st) {
+hipError_t launch1(KdParams p, hipStream_t st) {
     const size_t lds = (size_t)p.k * 16 + (p.bits ? ((size_t)p.V + 95) / 32 * 4 : 0);
     auto kern = &k_distill<DT, NT, VPT, BIG, OPEN>;
     if (lds > 64 * 1024) {                                  // 2^20 classes: 128 KB of bits
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL(kern, dim3((unsigned)p.N), dim3(NT), lds, st, p);
-    return hipGetLastError();
+    constexpr int64_t MOST = 0xffffffffu / NT;              // a launch's threads are counted in 32 bits
+    for (; p.n0 < p.N; p.n0 += MOST) {
+        const int64_t rows = p.N - p.n0 < MOST ? p.N - p.n0 : MOST;
+        hipLaunchKernelGGL(kern, dim3((unsigned)rows), dim3(NT), lds, st, p);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 template <int DT, bool OPEN>
 hipError_t launch(const KdParams& p, hipStream_t st) {
@@ -425,7 +432,7 @@ extern "C" int gr_distill_topk(gr_ctx* ctx, const void* z, int dtype, int64_t N,
     if (((uintptr_t)z | (uintptr_t)grad) % size(dtype) || (uintptr_t)value % size(value_type))
         return gr_fail(ctx, GR_EINVAL, "gr_distill_topk: misaligned tensor");
     if (grad == z && ldg != ldz) return gr_fail(ctx, GR_EINVAL, "gr_distill_topk: in place needs ldg == ldz");
-    KdParams p = {z, grad, index, value, value_type, teacher_lse, grad_loss, loss, N, ldz, ldg, ld_top, V, k, tau, 1.0 / (double)tau, 0, 0, V <= (1 << 20)};
+    KdParams p = {z, grad, index, value, value_type, teacher_lse, grad_loss, loss, N, ldz, ldg, ld_top, 0, V, k, tau, 1.0 / (double)tau, 0, 0, V <= (1 << 20)};
     const double c = 1.4426950408889634074 / (double)tau;
     p.c_hi = (float)c;
     if ((double)p.c_hi >= c) p.c_hi = nextafterf(p.c_hi, 0.f);

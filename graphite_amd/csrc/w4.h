@@ -956,12 +956,23 @@ static hipError_t launch_rows(const W4Params& p, hipStream_t st) {
 template <int DT, int ST, bool HALF, bool GRAD, int TM, int TN, int WM, int WN, int KS>
 static hipError_t launch_gemm(const W4Params& p, hipStream_t st) {
     using G = W4Gemm<DT, GRAD, TM, TN, WM, WN, KS>;
+    typedef typename W4Type<DT>::T T;
     auto kern = &k_w4_gemm<DT, ST, HALF, GRAD, TM, TN, WM, WN, KS>;
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, G::LDS);
     if (e != hipSuccess) return e;
-    const int64_t blocks = (int64_t)((p.R + G::BM - 1) / G::BM) * ((p.N + G::BN - 1) / G::BN);
-    hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(G::NT), G::LDS, st, p);
-    return hipGetLastError();
+    const int64_t across = (p.R + G::BM - 1) / G::BM;
+    const int64_t most = 0xffffffffu / G::NT / across * G::BN;          // rows of a launch, whose threads are counted in 32 bits
+    for (int64_t n0 = 0; n0 < p.N; n0 += most) {
+        W4Params q = p;
+        q.N = p.N - n0 < most ? p.N - n0 : most;
+        q.x = (const T*)p.x + n0 * p.ldx;
+        q.y = (T*)p.y + n0 * p.ldy;
+        if (p.gate) q.gate = (const T*)p.gate + n0 * p.ldg;
+        hipLaunchKernelGGL(kern, dim3((unsigned)(across * ((q.N + G::BN - 1) / G::BN))), dim3(G::NT), G::LDS, st, q);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 template <int DT, int ST, bool HALF, bool GRAD>
 static hipError_t launch_typed(const W4Params& p, hipStream_t st) {

@@ -74,6 +74,9 @@ extern "C" int gr_w4_create(gr_ctx* ctx, const uint8_t* q, int64_t ldq, const vo
     const int G = (int)(((int64_t)K + group - 1) / group);
     if (ldq < ((int64_t)K + 1) / 2 || lds < G || (zeros && ldz < G))
         return gr_fail(ctx, GR_EINVAL, "gr_w4_create: a row stride is shorter than its row");
+    // the packing kernels take a thread per eight weights, which a launch counts in 32 bits
+    if (((int64_t)M + 127) / 128 * 128 * (((int64_t)K + 127) / 128 * 128) / 8 > 0xffffff00ll)
+        return gr_fail(ctx, GR_EINVAL, "gr_w4_create: %d x %d are too many weights", M, K);
     hipStream_t st = (hipStream_t)stream;
     gr_w4* w = new (std::nothrow) gr_w4();
     if (!w) return gr_fail(ctx, GR_ENOMEM, "gr_w4_create: out of host memory");
@@ -94,7 +97,6 @@ extern "C" int gr_w4_create(gr_ctx* ctx, const uint8_t* q, int64_t ldq, const vo
     w->zeros = (uint8_t*)m; m += zsz;
     const int64_t nd = (int64_t)(pk / 4), ns = (int64_t)G * w->Mp;
     const dim3 gp((unsigned)((nd + 255) / 256)), gs((unsigned)((ns + 255) / 256));
-    if (nd / 256 >= INT_MAX || ns / 256 >= INT_MAX) { gr_w4_destroy(w); return gr_fail(ctx, GR_EINVAL, "gr_w4_create: too many weights"); }
     hipLaunchKernelGGL(k_w4_pack<false>, gp, dim3(256), 0, st, q, ldq, M, K, w->Kp / W4_CHUNK, nd, (unsigned*)w->pack);
     if (input_grad)
         hipLaunchKernelGGL(k_w4_pack<true>, gp, dim3(256), 0, st, q, ldq, M, K, w->Mp / W4_CHUNK, nd, (unsigned*)w->packT);

@@ -286,7 +286,8 @@ typedef struct gr_w4 gr_w4;
  *   zeros   [out_features][G] bytes 0..15 (the low four bits count), rows ldz bytes apart; NULL = 8 everywhere
  *   bias    float32 [out_features] or NULL
  *   group   a multiple of 32; the last group of a row may be short, and group may exceed in_features (one scale per row)
- *   input_grad != 0 keeps a second, transposed copy of the 4-bit weights for gr_linear_w4_input_grad. */
+ *   input_grad != 0 keeps a second, transposed copy of the 4-bit weights for gr_linear_w4_input_grad.
+ * At most 2^35 - 2048 weights, both sides rounded up to multiples of 128. */
 int gr_w4_create(gr_ctx* ctx, const uint8_t* q, int64_t ldq, const void* scales, int scale_type, int64_t lds, const uint8_t* zeros,
                  int64_t ldz, const float* bias, int out_features, int in_features, int group, int input_grad, void* stream,
                  gr_w4** out);

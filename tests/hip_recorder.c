@@ -7,7 +7,7 @@
 #include <stdint.h>
 #include <string.h>
 
-enum { MAX_KERNELS = 8192, MAX_LAUNCHES = 65536 };
+enum { MAX_KERNELS = 1 << 18, MAX_LAUNCHES = 65536 };
 typedef struct { const void* fn; const char* name; } Kernel;
 typedef struct { const char* name; unsigned grid[3], block[3]; size_t lds; uint64_t arg; } Launch;
 static Kernel kernels[MAX_KERNELS];

@@ -283,3 +283,14 @@ def test_gradient_where_the_target_does_not_add_up_to_one(case, v, dtype):
         fd = np.where(np.isfinite(zd[:, i]), scale * (up - down) / (2 * h), 0.0)
         tol = scale * 2 * (1e-6 + 4 * 1100 * 2.0 ** -24) + np.abs(gd[:, i]) * torch.finfo(dtype).eps / 2
         assert (np.abs(gd[:, i] - fd) <= tol).all()
+
+
+def test_rows_past_one_launch():
+    """2^26 rows of two classes are more threads than one launch counts: every row as in a small batch."""
+    n, t = 2 ** 26 + 1024, 1024
+    z, top, _ = _inputs(t, 2, 1, F16, 33)
+    want_l, want_g = topk_distill(z, top.index, top.value, 1.0, top.lse)
+    loss, grad = topk_distill(z.repeat(n // t, 1), top.index.repeat(n // t, 1), top.value.repeat(n // t, 1), 1.0, top.lse.repeat(n // t))
+    assert torch.equal(loss.view(-1, t), want_l.expand(n // t, t)) and torch.equal(grad.view(-1, t, 2), want_g.expand(n // t, t, 2))
+    del loss, grad
+    torch.cuda.empty_cache()

@@ -381,3 +381,22 @@ def _packed(m, k):
     groups = -(-k // 32)
     s = (torch.rand((m, groups), generator=g) * 0.02 + 0.001).to(F16)
     return q.cuda(), s.cuda(), torch.randint(0, 16, (m, groups), generator=g, dtype=torch.uint8).cuda()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16], ids=["f32", "f16"])
+def test_rows_past_one_launch(dtype):
+    """2^30 rows of one input and one output: more workgroups of the tiled kernels than one launch counts threads for."""
+    n = 2 ** 30 + 300
+    layer, w, _ = _layer(1, 1, 32, sdt=F16, seed=2)
+    rows = torch.tensor([0, 1, 2 ** 29, 2 ** 30 - 129, 2 ** 30 - 128, 2 ** 30 - 1, 2 ** 30, n - 2, n - 1], device="cuda")
+    x = torch.zeros(n, 1, device="cuda", dtype=dtype)
+    vals = torch.randn(len(rows), 1, generator=torch.Generator().manual_seed(3)).to(dtype)
+    x[rows] = vals.cuda()
+    for run in (layer.forward, layer.input_grad):
+        y = run(x)
+        expect = vals.double().numpy() * w[0, 0]
+        assert (np.abs(y[rows].cpu().double().numpy() - expect) <= _tol(expect, np.abs(expect), 1, dtype, 2.0 ** -15)).all()
+        y[rows] = 0
+        assert not y.any()
+        del y
+    torch.cuda.empty_cache()
