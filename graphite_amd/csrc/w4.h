@@ -948,10 +948,14 @@ static hipError_t launch_rows(const W4Params& p, hipStream_t st) {
 }
 template <int DT, int ST, bool HALF, int NT, int MT, bool GRAD>
 static hipError_t launch_rows(const W4Params& p, hipStream_t st) {
-    if constexpr (GRAD) return launch_rows<DT, ST, HALF, NT, MT, 1, true>(p, st);
-    else if (p.gsteps % 4 == 0) return launch_rows<DT, ST, HALF, NT, MT, 1, false>(p, st);
-    else if (p.gsteps % 2 == 0) return launch_rows<DT, ST, HALF, NT, MT, 2, false>(p, st);
-    else return launch_rows<DT, ST, HALF, NT, MT, 4, false>(p, st);
+    if constexpr (GRAD) {
+        return launch_rows<DT, ST, HALF, NT, MT, 1, true>(p, st);
+    } else {
+        if (p.gsteps % 4 == 0) return launch_rows<DT, ST, HALF, NT, MT, 1, false>(p, st);
+        if constexpr (!(HALF && NT == 4))                  // that one is not taken for groups of odd multiples of 32
+            if (p.gsteps % 2) return launch_rows<DT, ST, HALF, NT, MT, 4, false>(p, st);
+        return launch_rows<DT, ST, HALF, NT, MT, 2, false>(p, st);
+    }
 }
 template <int DT, int ST, bool HALF, bool GRAD, int TM, int TN, int WM, int WN, int KS>
 static hipError_t launch_gemm(const W4Params& p, hipStream_t st) {
@@ -991,14 +995,13 @@ static hipError_t launch_typed(const W4Params& p, hipStream_t st) {
     constexpr bool F32 = DT == GR_DT_F32, F16 = DT == GR_DT_F16;
     constexpr Cost fwd[7] = {F32 ? Cost{0.05f, 0.16f, 0.67f} : Cost{0.05f, 0.09f, 0.83f},      // row tiles x batch tiles: 1 x 1
                              F32 ? Cost{0.05f, 0.22f, 0.71f} : Cost{0.05f, 0.11f, 0.68f},      // 2 x 1
-                             F32 ? Cost{0.05f, 0.47f, 0.69f} : Cost{0.09f, 0.21f, 0.74f},      // 2 x 2
+                             Cost{0.09f, 0.21f, 0.74f},                                        // 2 x 2 (16-bit)
                              F32 ? Cost{0.30f, 0.59f, 0.60f} : Cost{0.18f, 0.31f, 0.57f},      // 4 x 2
-                             F32 ? Cost{2.64f, 2.69f, 0.75f} : Cost{2.32f, 0.58f, 1.25f},      // 4 x 4
+                             Cost{2.32f, 0.58f, 1.25f},                                        // 4 x 4 (16-bit)
                              F32 ? Cost{2.88f, 2.80f, 1.32f} : Cost{5.72f, 2.91f, 1.20f},      // tiled
                              Cost{2.67f, 1.39f, 1.50f}};                                       // tiled, half the batch rows (16-bit)
-    constexpr Cost grad[5] = {F32 ? Cost{0.05f, 0.28f, 0.72f} : Cost{0.05f, 0.20f, 0.77f},     // 2 x 1
+    constexpr Cost grad[4] = {F32 ? Cost{0.05f, 0.28f, 0.72f} : Cost{0.05f, 0.20f, 0.77f},     // 2 x 1
                               F32 ? Cost{0.05f, 0.34f, 0.70f} : Cost{0.05f, 0.28f, 0.72f},     // 4 x 1
-                              F32 ? Cost{0.06f, 0.67f, 0.61f} : Cost{0.15f, 0.49f, 0.63f},     // 4 x 2
                               F32 ? Cost{0.80f, 1.08f, 1.26f} : Cost{1.35f, 0.78f, 1.15f},     // 8 x 2
                               F32 ? Cost{2.19f, 3.97f, 1.72f} : F16 ? Cost{0.69f, 2.76f, 1.82f} : Cost{4.08f, 3.20f, 1.43f}};  // tiled
     auto time = [&](const Cost& c, int rows, int cols, bool large, float slower) {          // of workgroups of rows x cols outputs
@@ -1019,32 +1022,32 @@ static hipError_t launch_typed(const W4Params& p, hipStream_t st) {
         consider(0, time(fwd[0], 16, 16, false, 1.f));
         consider(1, time(fwd[1], 32, 16, false, 1.f));
         if (p.N > 16) {
-            consider(2, time(fwd[2], 32, 32, false, 1.f));
+            if (!F32) consider(2, time(fwd[2], 32, 32, false, 1.f));
             consider(3, time(fwd[3], 64, 32, false, 1.f));
             // 4 x 4 spills registers where a chunk has several groups or rows begin inside a dword: measured against the above
-            consider(4, time(fwd[4], 64, 64, true, (odd ? 1.4f : p.gsteps % 4 ? 1.1f : 1.f) * (HALF ? 1.5f : 1.f)));
+            if (!F32 && !(HALF && odd)) consider(4, time(fwd[4], 64, 64, true, (odd ? 1.4f : p.gsteps % 4 ? 1.1f : 1.f) * (HALF ? 1.5f : 1.f)));
             if (F32 || !odd) consider(5, time(fwd[5], 128, tiled_cols, true, odd ? 1.2f : 1.f));
             if (!F32) consider(6, time(fwd[6], 128, 128, true, odd ? 1.1f : 1.f));
         }
         if (best == 0) return launch_rows<DT, ST, HALF, 1, 1, GRAD>(p, st);
         if (best == 1) return launch_rows<DT, ST, HALF, 1, 2, GRAD>(p, st);
-        if (best == 2) return launch_rows<DT, ST, HALF, 2, 2, GRAD>(p, st);
+        if constexpr (!F32) {
+            if (best == 2) return launch_rows<DT, ST, HALF, 2, 2, GRAD>(p, st);
+            if (best == 4) return launch_rows<DT, ST, HALF, 4, 4, GRAD>(p, st);
+        }
         if (best == 3) return launch_rows<DT, ST, HALF, 2, 4, GRAD>(p, st);
-        if (best == 4) return launch_rows<DT, ST, HALF, 4, 4, GRAD>(p, st);
     } else {
         // a workgroup's row tiles share one group: its scales go to the activations
         const int most = p.gsteps % 4 == 0 ? 8 : p.gsteps % 2 == 0 ? 4 : 2;
         consider(0, time(grad[0], 32, 16, false, 1.f));
         if (most >= 4) consider(1, time(grad[1], 64, 16, false, 1.f));
         if (p.N > 16) {
-            if (most >= 4) consider(2, time(grad[2], 64, 32, false, 1.f));
-            if (most == 8) consider(3, time(grad[3], 128, 32, true, 1.f));
-            consider(4, time(grad[4], 128, tiled_cols, true, 1.f));
+            if (most == 8) consider(2, time(grad[2], 128, 32, true, 1.f));
+            consider(3, time(grad[3], 128, tiled_cols, true, 1.f));
         }
         if (best == 0) return launch_rows<DT, ST, HALF, 1, 2, GRAD>(p, st);
         if (best == 1) return launch_rows<DT, ST, HALF, 1, 4, GRAD>(p, st);
-        if (best == 2) return launch_rows<DT, ST, HALF, 2, 4, GRAD>(p, st);
-        if (best == 3) return launch_rows<DT, ST, HALF, 2, 8, GRAD>(p, st);
+        if (best == 2) return launch_rows<DT, ST, HALF, 2, 8, GRAD>(p, st);
     }
     if constexpr (DT == GR_DT_F32 || (GRAD && DT == GR_DT_F16)) return launch_gemm<DT, ST, HALF, GRAD, 4, 2, 2, 4, 1>(p, st);
     else if constexpr (GRAD) return launch_gemm<DT, ST, HALF, GRAD, 4, 4, 2, 4, 1>(p, st);

@@ -18,6 +18,8 @@ static uintptr_t next = (uintptr_t)1 << 44;
 static struct { dim3 g, b; size_t lds; hipStream_t st; } conf;
 
 int rec_device(void) { return device; }
+int rec_kernels(void) { return nkernels; }
+const char* rec_kernel(int i) { return kernels[i].name; }
 int rec_launches(void) { return nlaunches; }
 void rec_clear(void) { nlaunches = 0; }
 const char* rec_name(int i) { return launches[i].name; }

@@ -30,7 +30,7 @@ class Recorder:
 
     def __init__(self, so):
         self.hip = C.CDLL(so, mode=C.RTLD_GLOBAL)        # before the library: its symbols are found first
-        self.hip.rec_name.restype = C.c_char_p
+        self.hip.rec_name.restype = self.hip.rec_kernel.restype = C.c_char_p
         self.hip.rec_grid.restype = self.hip.rec_block.restype = C.POINTER(C.c_uint)
         self.hip.rec_lds.restype = C.c_size_t
         self.hip.rec_arg.restype = C.c_uint64
@@ -51,6 +51,10 @@ class Recorder:
         assert rc == 0, (rc, self.lib.gr_last_error(ctx))
         self.hip.rec_clear()
         return w
+
+    def kernels(self):
+        """Names of every kernel that was registered."""
+        return [self.hip.rec_kernel(i).decode() for i in range(self.hip.rec_kernels())]
 
     def launches(self):
         """[(kernel, grid, block, LDS bytes, first argument's first eight bytes)] since the last call."""

@@ -1,5 +1,6 @@
 """Host side of the 4-bit layers' and the distillation loss' C entries, on the CPU (hip_recorder.c stands in for the runtime)."""
 import hip_recorder
+import w4_cases
 
 
 def test_destroying_a_layer_leaves_the_current_device(tmp_path):
@@ -59,3 +60,37 @@ for m, k in ((1 << 17, 1 << 18), (1, (1 << 28) + 1), ((1 << 31) - 400, 64), (1 <
     result.append([rc, bool(rec.launches()), bool(w.value)])
 """)
     assert got == [[-1, False, False]] * 3 + [[0, True, True]] * 2
+
+
+CHOICES = """
+import re
+def parse(name):
+    a = [int(v) for v in re.findall("L[ib]([0-9]+)E", name)]
+    if "k_w4_rows" in name:
+        dt, st, half, nt, mt, gs, d, grad = a
+        return [["rows", nt, mt, gs], grad, dt, half]
+    dt, st, half, grad, tm, tn, wm, wn, ks = a
+    return [["tiled", tn, ks], grad, dt, half]
+ctx, p, chosen = rec.context(), 1 << 40, []
+for kernel, grad, n, k, m, group, t in cases:
+    w = rec.layer(ctx, m, k, group)
+    dt, half = ("f32", "bf16", "f16").index(t.rstrip("*")), t.endswith("*")
+    c = m if grad else k
+    x, ld = p + (2 if half else 0), c if dt == 0 else c + (c + half) % 2
+    if grad: rc = rec.lib.gr_linear_w4_input_grad(ctx, w, x, dt, n, ld, None, 0, p, k, None)
+    else: rc = rec.lib.gr_linear_w4(ctx, w, x, dt, n, ld, 0, p, m, None)
+    names = [l[0] for l in rec.launches()]
+    chosen.append([rc, len(names), parse(names[0])])
+result = [chosen, [parse(n) for n in rec.kernels() if "k_w4_rows" in n or "k_w4_gemm" in n]]
+"""
+
+
+def test_every_kernel_of_the_layers_has_its_case(tmp_path):
+    """The sizes of w4_cases.py take the kernels they name, and there is no kernel that none of them takes."""
+    chosen, built = hip_recorder.run(tmp_path, f"cases = {w4_cases.FLAT!r}\n" + CHOICES)
+    as_set = lambda rows: {(tuple(k), *rest) for k, *rest in rows}
+    for case, (rc, count, got) in zip(w4_cases.FLAT, chosen):
+        kernel, grad, *_, t = case
+        dt = ("f32", "bf16", "f16").index(t.rstrip("*"))
+        assert rc == 0 and count == 1 and got == [list(kernel), int(grad), dt, int(t.endswith("*"))], (w4_cases.label(case), got)
+    assert as_set(g for _, _, g in chosen) == as_set(built)
