@@ -9,7 +9,8 @@
 //             matrix instruction each.
 //   gradient  the scale changes along the sum (it belongs to m), so it goes to a factor: to gy in the few-row kernel (gy * s in
 //             f32, its rows sharing one group), to the weights in the tiled one ((q - z) * s in f32, any mix of groups).  That
-//             factor is cut into two (16-bit types, 2^-15 relative: a 64th of their own rounding) or three (f32) bf16 pieces.
+//             factor is cut into two (16-bit types) or three (f32) bf16 pieces.  A product is off by at most 2^-15 in 16-bit
+//             types -- a 128th of bf16's own rounding, a 16th of f16's -- and 1.5 * 2^-23 in f32, a third of it the factor's rounding.
 // Sums are f32 throughout; only the stored output is rounded to the tensors' type.
 //
 // Packed layout ("tiles"): 16 rows x 128 contraction steps = 64 lanes x 16 bytes = 1 KB, the operand of four matrix
@@ -99,8 +100,12 @@ __device__ __forceinline__ w4_f16x8 w4_ints_f16(unsigned w, float zk) {
     return o.v;
 }
 // v = p0 + p1 (+ p2) with bf16 pieces, each cut from what the ones before leave, the last one of two rounded: three pieces are
-// exact, two leave at most 2^-15 |v|.  An infinity stays in p0 alone.
-template <int P>
+// exact, two leave at most 2^-16 |v|.  An infinity stays in p0 alone.
+// NEAR, for products of pieces of which the smallest are left out: p0 is rounded to nearest (values next to float32's largest,
+// LARGE, to bf16's), so that what it leaves has either sign and is at most 2^-8 |v|, half of what a cut leaves, always with the
+// sign of v.  Three pieces are exact still, two leave 2^-17 |v|, of an f16 value (not LARGE) nothing.  Infinities and NaNs leave
+// NaN or infinity in p1.
+template <int P, bool NEAR = false, bool LARGE = true>
 __device__ __forceinline__ void w4_pieces(const float (&v)[8], w4_bf16x8 (&out)[P]) {
     union { unsigned u[4]; w4_bf16x8 b; } o[P];
 #pragma unroll
@@ -108,16 +113,21 @@ __device__ __forceinline__ void w4_pieces(const float (&v)[8], w4_bf16x8 (&out)[
         float r[2] = {v[2 * h], v[2 * h + 1]};
 #pragma unroll
         for (int p = 0; p < P; p++) {
-            if (p == 1 && P == 2) {
+            float t[2] = {r[0], r[1]};
 #pragma unroll
-                for (int i = 0; i < 2; i++) r[i] = __uint_as_float(__float_as_uint(r[i]) + 0x8000u);
+            for (int i = 0; i < 2; i++) {
+                if (p == 1 && P == 2 && !(NEAR && !LARGE)) t[i] = __uint_as_float(__float_as_uint(r[i]) + 0x8000u);
+                if (p == 0 && NEAR) {
+                    if (LARGE) t[i] = __builtin_amdgcn_fmed3f(r[i], -0x1.fefffep127f, 0x1.fefffep127f);
+                    t[i] = __uint_as_float(__float_as_uint(t[i]) + 0x8000u);
+                }
             }
-            o[p].u[h] = w4_pack_hi(r[0], r[1]);
+            o[p].u[h] = w4_pack_hi(t[0], t[1]);
             if (p == P - 1) continue;
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const float d = r[i] - __uint_as_float(__float_as_uint(r[i]) & 0xffff0000u);
-                r[i] = p == 0 && __builtin_fabsf(r[i]) == __builtin_inff() ? 0.f : d;
+                const float d = r[i] - __uint_as_float(__float_as_uint(t[i]) & 0xffff0000u);
+                r[i] = !NEAR && p == 0 && __builtin_fabsf(r[i]) == __builtin_inff() ? 0.f : d;
             }
         }
     }
@@ -478,7 +488,10 @@ __global__ __launch_bounds__(w4_rows_waves(NT) * 64) void k_w4_rows(W4Params p) 
 template <int DT, bool GRAD> struct W4Pieces {          // pieces of the weights and of the activations
     static constexpr int W = !GRAD ? 1 : DT == GR_DT_F32 ? 3 : 2;
     static constexpr int X = DT == GR_DT_F32 ? 3 : GRAD && DT == GR_DT_F16 ? 2 : 1;
-    static constexpr int TOP = W > X ? W : X;           // products i, j with i + j < TOP count
+    // Products of pieces i, j with i + j < TOP count.  What the gradients leave out is at most 2^-23 of |w x| in f32 (1 x 2 and
+    // 2 x 1: 2^-8 of one factor, 2^-16 of the other), 2^-16 in f16 (1 x 1; with the weight's rest 1.5 * 2^-16), with either sign.
+    static constexpr int TOP = W > X ? W : X;
+    static constexpr bool NEAR = W > 1 && X > 1;
     static constexpr int PROD = !GRAD ? X : DT == GR_DT_F32 ? 6 : DT == GR_DT_F16 ? 3 : 2;
 };
 template <int DT, bool GRAD, int TM, int TN, int WM, int WN, int KS>
@@ -605,7 +618,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
                 f[2 * q + 1] *= sc[2 * q + 1];
             }
             w4_bf16x8 pc[P::W];
-            w4_pieces<P::W>(f, pc);
+            w4_pieces<P::W, P::NEAR>(f, pc);
 #pragma unroll
             for (int q = 0; q < P::W; q++) {
                 c.b = pc[q];
@@ -622,7 +635,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_w4_gemm(W4Params p) {
             float f[8];
             xreg[v].get(f);
             w4_bf16x8 pc[P::X];
-            w4_pieces<P::X>(f, pc);
+            w4_pieces<P::X, P::NEAR, DT == GR_DT_F32>(f, pc);
 #pragma unroll
             for (int q = 0; q < P::X; q++) {
                 Frag c;

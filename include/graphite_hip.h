@@ -300,8 +300,8 @@ int gr_linear_w4(gr_ctx* ctx, const gr_w4* w, const void* x, int dtype, int64_t 
                  void* stream);
 /* grad_x[n,k] = sum_m grad_y[n,m] * (q[m,k] - z[m,k / group]) * s[m,k / group], 0 where gate[n,k] <= 0 (gate: the rectified
  * activation the layer read, same type as grad_x, rows ldgate apart; NULL = no gate).  The layer's own ReLU, if it had one,
- * is the caller's to apply to grad_y.  Same promises as gr_linear_w4 (the factor grad_y * s is rounded to float32, for 16-bit
- * types to 2^-15); a row of grad_y with an infinity or NaN gives a row of infinities and NaNs.  The weights are frozen: no
+ * is the caller's to apply to grad_y.  Same promises as gr_linear_w4, but for the products: each is off by at most
+ * 1.5 * 2^-23 of itself in float32 and 2^-15 in the 16-bit types, with either sign; a row of grad_y with an infinity or NaN gives a row of infinities and NaNs.  The weights are frozen: no
  * gradient is formed for them. */
 int gr_linear_w4_input_grad(gr_ctx* ctx, const gr_w4* w, const void* grad_y, int dtype, int64_t N, int64_t ldgy, const void* gate,
                             int64_t ldgate, void* grad_x, int64_t ldgx, void* stream);

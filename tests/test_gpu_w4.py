@@ -400,3 +400,91 @@ def test_rows_past_one_launch(dtype):
         assert not y.any()
         del y
     torch.cuda.empty_cache()
+
+
+def _weights_of(rows, m, k, group):
+    """(LinearW4 [m, k], its float64 weights) that are zero but for `rows`: {row: (code - zero point, scales [groups])}."""
+    groups = -(-k // group)
+    q, z, s = np.full((m, k + k % 2), 8, np.uint8), np.full((m, groups), 8, np.uint8), np.ones((m, groups), np.float32)
+    for r, (c, scales) in rows.items():
+        z[r] = 8 if abs(c) <= 7 else 2
+        q[r], s[r] = int(z[r, 0]) + c, scales
+    w = (q[:, :k].astype(np.float64) - z.astype(np.float64)[:, np.arange(k) // group]) * s.astype(np.float64)[:, np.arange(k) // group]
+    packed = q[:, 0::2] | (q[:, 1::2] << 4)
+    return LinearW4(torch.from_numpy(packed).cuda(), torch.from_numpy(s).cuda(), torch.from_numpy(z).cuda(), group=group, in_features=k), w
+
+
+# The sizes take the LDS-tiled gradient (w4_cases.py) or the few-row one.
+PRODUCTS = [(723, 1827, 639), (2, 40, 70)]
+
+
+@pytest.mark.parametrize("n,k,m", PRODUCTS, ids=["tiled", "rows"])
+def test_single_products_of_the_float32_gradient(n, k, m):
+    """Two weight rows count and nearly cancel: gy5 w5 - w6 with w6 the float32 next to gy5 w5 and gy6 = -1, a product that three
+    pieces hold exactly.  What is left shows the error of the first, promised to be within 1.5 * 2^-23 of it; the large pieces of
+    both meet in one instruction, so the twelve additions, each off by 2^-23, stay below 2^-5.  w5 = 1 + a 2^-15 and
+    gy5 = 1 + 2^-8 + b 2^-23, a and b < 256: a cut into pieces that leaves out a 2^-15 times b 2^-23 is off by up to 2^-22."""
+    g = np.random.default_rng(0)
+    groups = -(-k // 32)
+    a = np.concatenate([[255, 254, 253, 129], g.integers(1, 256, max(0, groups - 4))])[:groups]
+    b = np.concatenate([[255, 128], g.integers(1, 256, max(0, n - 2))])[:n]
+    worst = 0.0
+    for bb in sorted(set(b.tolist()))[-8:]:
+        s5 = (1 + a * 2.0 ** -15).astype(np.float32)
+        gy = np.zeros((n, m))
+        gy[:, 5], gy[:, 6] = 1 + 2.0 ** -8 + bb * 2.0 ** -23, -1.0
+        layer, w = _weights_of({5: (1, s5), 6: (1, (gy[0, 5] * s5.astype(np.float64)).astype(np.float32))}, m, k, 32)
+        gx = layer.input_grad(torch.from_numpy(gy).float().cuda()).double().cpu().numpy()
+        err, mag = np.abs(gx - gy @ w), gy[0, 5] * np.abs(w[5])
+        worst = max(worst, float((err / mag).max()))
+    assert worst <= 1.5 * 2.0 ** -23 + 12 * 2.0 ** -28, worst * 2.0 ** 23
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("n,k,m", PRODUCTS + [(419, 3884, 619)], ids=["tiled", "rows", "tiled-bf16"])
+def test_single_products_of_the_16_bit_gradients(n, k, m, dtype):
+    """Two weight rows count and nearly cancel: gy5 w5 - gy6 w6 with w6 the 16-bit value next to gy5 w5 / gy6 and gy6 a power of
+    two, a product that two pieces hold exactly.  What is left shows the error of the first, promised to be within 2^-15 of it."""
+    g = np.random.default_rng(1)
+    groups = -(-k // 32)
+    s = np.concatenate([[0.011451721], g.uniform(0.01, 0.02, max(0, groups - 1))])[:groups].astype(np.float32)
+    a = float(torch.tensor(1.0537109375).to(dtype))
+    prod = a * 11.0 * s.astype(np.float64)
+    e = np.floor(np.log2(prod)) - 15
+    s6 = (np.round(prod / 2.0 ** e) * 2.0 ** e).astype(np.float32)
+    layer, w = _weights_of({5: (11, s), 6: (-1, s6)}, m, k, 32)
+    gy = np.zeros((n, m))
+    up = 2.0 ** (np.arange(n) % 4 + 8)
+    gy[:, 5], gy[:, 6] = a * up, up
+    gx = layer.input_grad(torch.from_numpy(gy).to(dtype).cuda()).double().cpu().numpy()
+    ref, mag = gy @ w, np.abs(gy) @ np.abs(w)
+    tol = mag / 2 * 1.001 * 2.0 ** -15 + mag * 8 * 2.0 ** -23 + np.abs(ref) * torch.finfo(dtype).eps / 2 * 1.01 + 2.0 ** -25
+    assert (np.abs(gx - ref) <= tol).all(), (np.abs(gx - ref) / tol).max()
+
+
+@pytest.mark.parametrize("dtype,patterns", [(F32, (0x7f800001, 0x7fffffff, -1, -0x400000)), (BF16, (0x7f81, 0x7fff, -1, -0x40)),
+                                            (F16, (0x7c01, 0x7fff, -1, -0x200))], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n,k,m", PRODUCTS + [(419, 3884, 619), (2060, 678, 1604)], ids=["tiled", "rows", "tiled-bf16", "tiled-forward"])
+def test_every_nan_stays_one(n, k, m, dtype, patterns):
+    """NaNs of any payload: the pieces and halves that the kernels make of them must not turn into numbers."""
+    layer, _, _ = _layer(m, k, 32, seed=15)
+    ints = torch.int32 if dtype == F32 else torch.int16
+    for run, c in ((layer.forward, k), (layer.input_grad, m)):
+        x = torch.randn((n, c), generator=torch.Generator().manual_seed(1)).to(dtype)
+        rows = min(n, len(patterns))
+        for i in range(rows):
+            x.view(ints)[i, (7 * i + 5) % c] = patterns[i]
+        y = run(x.cuda())
+        assert bool(torch.isnan(y[:rows]).all()) and bool(torch.isfinite(y[rows:]).all())
+
+
+@pytest.mark.parametrize("n,k,m", PRODUCTS, ids=["tiled", "rows"])
+def test_float32_gradient_extremes(n, k, m):
+    """grad_y at float32's largest values and at 2^-100: rounding a piece must not overflow, nor may the low pieces be lost."""
+    layer, w = _weights_of({5: (3, np.full(-(-k // 32), 2.0 ** -6, np.float32))}, m, k, 32)
+    gy = np.zeros((n, m))
+    top = float(torch.finfo(F32).max)
+    gy[:, 5] = np.resize([top, -top, top * (1 - 2.0 ** -9), (1 + 2.0 ** -9) * 2.0 ** -100], n)
+    gx = layer.input_grad(torch.from_numpy(gy).float().cuda()).double().cpu().numpy()
+    ref = torch.from_numpy(gy).float().double().numpy() @ w
+    assert (np.abs(gx - ref) <= 2.0 ** -21 * np.abs(ref)).all()
