@@ -141,6 +141,7 @@ __device__ __forceinline__ void w4_pieces(const float (&v)[8], w4_bf16x8 (&out)[
 // before they are used; every dword read holds an element of the row.  2048 rows 4095 -> 4096 bf16: 226 us with the long loads,
 // 126 so (4096 -> 4096: 100).
 typedef unsigned w4_u32x4_u __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned w4_u32x4_h __attribute__((ext_vector_type(4), aligned(2)));
 template <int DT, bool HALF = false> struct W4Raw {
     static constexpr int Q = DT == GR_DT_F32 ? 2 : 1;
     typedef typename W4Type<DT>::T T;
@@ -183,10 +184,15 @@ template <int DT, bool HALF = false> struct W4Raw {
         union { w4_u32x4 q[Q]; T t[8]; unsigned u[4 * Q]; } u;
         if (wide) {
             const T* from = count < 8 ? src + (count - 8) : src;
-            load(from);
-            settle((uintptr_t)from & 2 ? 16 : 0);
+            if constexpr (HALF) {
+                load(from);
+                settle((uintptr_t)from & 2 ? 16 : 0);
 #pragma unroll
-            for (int i = 0; i < Q; i++) u.q[i] = q[i];
+                for (int i = 0; i < Q; i++) u.q[i] = q[i];
+            } else {                                                            // rows of an odd length end inside a dword
+#pragma unroll
+                for (int i = 0; i < Q; i++) u.q[i] = *(const w4_u32x4_h*)(from + i * (16 / (int)sizeof(T)));
+            }
             const int sh = count >= 8 ? 0 : 8 - count;                          // elements to move by; 8 and more leave nothing
             constexpr int W = 4 / (int)sizeof(T);                               // elements of a dword
 #pragma unroll
