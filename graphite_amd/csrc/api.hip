@@ -514,8 +514,7 @@ static int model_input_grad(gr_ctx* ctx, gr_model* m, const char* who, const flo
     const int ncls = gr_model_num_classes(m);
     // the pass keeps every activation: ~0.8 MB per image for GTSRBNet, ~17 MB for WideResNet-34-10
     int64_t cap = (int64_t)(ctx->ws_limit / (net_grad_workspace_bytes(m, 64) / 64 + 1));
-    if (cap < 1) cap = 1;
-    if (cap > 1024) cap = 1024;
+    cap = cap < 4 ? 4 : cap > 1024 ? 1024 : cap / 4 * 4;    // by fours: a row of logits keeps its place within 16 bytes in every chunk
     int chunk = N < cap ? N : (int)cap;
     if (chunk <= 0) return GR_OK;
     int rc = gr_ws_reserve(ctx, net_grad_workspace_bytes(m, chunk), stream);

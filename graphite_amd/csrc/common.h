@@ -135,9 +135,14 @@ int net_pg_out_size(const gr_model*);
 struct NetSoftTarget { const int64_t* index; const float* value; const float* lse; int k; int64_t ld_top; float tau; float* loss; };
 int net_input_grad(gr_ctx*, gr_model*, const float* x_chw, int N, int target, const NetSoftTarget* soft, float* logits_or_null,
                    float* grad_x, char* ws, size_t ws_bytes, hipStream_t);
+size_t net_grad_workspace_bytes(const gr_model*, int N);
 
 // ---- w4.hip ----
 gr_ctx* w4_ctx(const gr_w4*);
 int w4_out_features(const gr_w4*);
 int w4_in_features(const gr_w4*);
-size_t net_grad_workspace_bytes(const gr_model*, int N);
+// gr_linear_w4, gr_linear_w4_input_grad of float32 rows inside a model: one order of summation whatever N is, so that what an
+// image gets does not depend on the chunk it is in
+int w4_model_forward(gr_ctx*, const gr_w4*, const float* x, int64_t N, int64_t ldx, int relu, float* y, int64_t ldy, hipStream_t);
+int w4_model_input_grad(gr_ctx*, const gr_w4*, const float* grad_y, int64_t N, int64_t ldgy, const float* gate, int64_t ldgate,
+                        float* grad_x, int64_t ldgx, hipStream_t);

@@ -1040,7 +1040,7 @@ static int gtsrb_fc(gr_ctx* ctx, gr_model* m, int l, const float* in, int N, flo
         in = tmp;
     }
     const int64_t K = l == 0 ? 2048 : 1024, M = l == 2 ? 43 : 1024;
-    return gr_linear_w4(ctx, m->w4[l], in, GR_DT_F32, N, K, l < 2, out, M, st);
+    return w4_model_forward(ctx, m->w4[l], in, N, K, l < 2, out, M, st);
 }
 
 static int gtsrb_forward(gr_ctx* ctx, gr_model* m, const float* x, int N, float* logits, float* ws, hipStream_t st) {
@@ -1161,7 +1161,7 @@ static int wrn_forward(gr_ctx* ctx, gr_model* m, const float* x, int N, float* l
     int C = m->ch[3];
     hipLaunchKernelGGL(k_avgpool, dim3((N * C + 255) / 256), dim3(256), 0, st, o, N, H * H, C, u);
     GR_HIP(ctx, hipGetLastError());
-    if (m->w4[0]) return gr_linear_w4(ctx, m->w4[0], u, GR_DT_F32, N, m->ch[3], 0, logits, m->ncls, st);
+    if (m->w4[0]) return w4_model_forward(ctx, m->w4[0], u, N, m->ch[3], 0, logits, m->ncls, st);
     return run_conv(ctx, m->wfc, u, N, 1, 1, nullptr, nullptr, logits, nullptr, false, false, st);
 }
 
@@ -1293,13 +1293,13 @@ int net_input_grad(gr_ctx* ctx, gr_model* m, const float* x, int N, int target, 
     if ((rc = gtsrb_fc(ctx, m, 2, f6, N, lgp, nullptr, st))) return rc;
     // ---- backward: every transposed layer gates its output with the ReLU of the activation it produces the gradient of ----
     if ((rc = logit_grad(ctx, m, lgp, N, target, soft, g64, st))) return rc;
-    if (m->w4[2]) { if ((rc = gr_linear_w4_input_grad(ctx, m->w4[2], g64, GR_DT_F32, N, 64, f6, 1024, gA, 1024, st))) return rc; }   // d f6
+    if (m->w4[2]) { if ((rc = w4_model_input_grad(ctx, m->w4[2], g64, N, 64, f6, 1024, gA, 1024, st))) return rc; }   // d f6
     else if ((rc = run_conv(ctx, m->gb[8], g64, N, 1, 1, nullptr, nullptr, gA, nullptr, false, false, st, f6))) return rc;
-    if (m->w4[1]) { if ((rc = gr_linear_w4_input_grad(ctx, m->w4[1], gA, GR_DT_F32, N, 1024, f5, 1024, gB, 1024, st))) return rc; }  // d f5
+    if (m->w4[1]) { if ((rc = w4_model_input_grad(ctx, m->w4[1], gA, N, 1024, f5, 1024, gB, 1024, st))) return rc; }  // d f5
     else if ((rc = run_conv(ctx, m->gb[7], gA, N, 1, 1, nullptr, nullptr, gB, nullptr, false, false, st, f5))) return rc;
     if (m->w4[0]) {                                                                                                                 // d p4
         float* chw = gB + (size_t)N * 1024;
-        if ((rc = gr_linear_w4_input_grad(ctx, m->w4[0], gB, GR_DT_F32, N, 1024, nullptr, 0, chw, 2048, st))) return rc;
+        if ((rc = w4_model_input_grad(ctx, m->w4[0], gB, N, 1024, nullptr, 0, chw, 2048, st))) return rc;
         if ((rc = fc5_order(ctx, chw, N, gA, false, st))) return rc;
     } else if ((rc = run_conv(ctx, m->gb[6], gB, N, 1, 1, nullptr, nullptr, gA, nullptr, false, false, st))) return rc;
     hipLaunchKernelGGL(k_maxpool2_relu_bwd, blocks((size_t)N * 2048), dim3(256), 0, st, a42, gA, N, 8, 8, 128, gB);      // d a42
@@ -1436,11 +1436,11 @@ static int wrn_input_grad(gr_ctx* ctx, gr_model* m, const float* x, int N, int t
     const int C3 = m->ch[3], P = H * H;
     hipLaunchKernelGGL(k_avgpool, blocks((size_t)N * C3), dim3(256), 0, st, OF, N, P, C3, pooled);
     float* lgp = logits_out ? logits_out : lg;
-    if (m->w4[0]) { if ((rc = gr_linear_w4(ctx, m->w4[0], pooled, GR_DT_F32, N, C3, 0, lgp, m->ncls, st))) return rc; }
+    if (m->w4[0]) { if ((rc = w4_model_forward(ctx, m->w4[0], pooled, N, C3, 0, lgp, m->ncls, st))) return rc; }
     else if ((rc = run_conv(ctx, m->wfc, pooled, N, 1, 1, nullptr, nullptr, lgp, nullptr, false, false, st))) return rc;
     // ---- backward ----
     if ((rc = logit_grad(ctx, m, lgp, N, target, soft, g64, st))) return rc;
-    if (m->w4[0]) { if ((rc = gr_linear_w4_input_grad(ctx, m->w4[0], g64, GR_DT_F32, N, 64, nullptr, 0, gA, C3, st))) return rc; }     // d pooled
+    if (m->w4[0]) { if ((rc = w4_model_input_grad(ctx, m->w4[0], g64, N, 64, nullptr, 0, gA, C3, st))) return rc; }     // d pooled
     else if ((rc = run_conv(ctx, m->wfcT, g64, N, 1, 1, nullptr, nullptr, gA, nullptr, false, false, st))) return rc;
     hipLaunchKernelGGL(k_pool_bn_relu_bwd, blocks((size_t)N * P * C3), dim3(256), 0, st, gA, OF, m->bnf.scale, N, P, C3, gY);
     for (size_t bi = nb; bi-- > 0;) {
@@ -1534,7 +1534,7 @@ int net_pg_local(gr_ctx* ctx, gr_model* m, const float* x, int N, float* local, 
         float* tmp = X; X = T1; T1 = tmp;
         H = Ho;
     }
-    if (m->w4[0]) return gr_linear_w4(ctx, m->w4[0], X, GR_DT_F32, (int64_t)N * H * H, m->bag_fc.CinT, 0, local, m->ncls, st);
+    if (m->w4[0]) return w4_model_forward(ctx, m->w4[0], X, (int64_t)N * H * H, m->bag_fc.CinT, 0, local, m->ncls, st);
     return run_conv(ctx, m->bag_fc, X, N, H, H, nullptr, nullptr, local, nullptr, false, false, st);
 }
 

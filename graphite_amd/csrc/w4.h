@@ -44,6 +44,7 @@ struct W4Params {
     const void* gate;        // [N][R], row stride ldg, or null (gradient): output 0 where gate <= 0
     int64_t N, ldx, ldy, ldg;
     int relu;
+    int waves;               // > 0: few-row kernels of that many waves, whatever N is: one order of summation (W4_MODEL_WAVES)
 };
 
 template <int DT> struct W4Type;
@@ -954,7 +955,7 @@ template <int DT, int ST, bool HALF, int NT, int MT, int GS, bool GRAD>
 static hipError_t launch_rows(const W4Params& p, hipStream_t st) {
     constexpr int D = DT == GR_DT_F32 || NT > 1 || GRAD || HALF ? 1 : 2;
     const int64_t blocks = (int64_t)((p.R + 16 * MT - 1) / (16 * MT)) * ((p.N + 16 * NT - 1) / (16 * NT));
-    int waves = blocks >= 2048 ? 4 : blocks >= 512 ? 8 : w4_rows_waves(NT);
+    int waves = p.waves > 0 ? p.waves : blocks >= 2048 ? 4 : blocks >= 512 ? 8 : w4_rows_waves(NT);
     if (waves > p.chunks) waves = p.chunks;
     const size_t lds = (size_t)waves * MT * NT * 1024;
     auto kern = &k_w4_rows<DT, ST, HALF, NT, MT, GS, D, GRAD>;
@@ -1045,8 +1046,8 @@ static hipError_t launch_typed(const W4Params& p, hipStream_t st) {
             consider(3, time(fwd[3], 64, 32, false, 1.f));
             // 4 x 4 spills registers where a chunk has several groups or rows begin inside a dword: measured against the above
             if (!F32 && !(HALF && odd)) consider(4, time(fwd[4], 64, 64, true, (odd ? 1.4f : p.gsteps % 4 ? 1.1f : 1.f) * (HALF ? 1.5f : 1.f)));
-            if (F32 || !odd) consider(5, time(fwd[5], 128, tiled_cols, true, odd ? 1.2f : 1.f));
-            if (!F32) consider(6, time(fwd[6], 128, 128, true, odd ? 1.1f : 1.f));
+            if (!p.waves && (F32 || !odd)) consider(5, time(fwd[5], 128, tiled_cols, true, odd ? 1.2f : 1.f));
+            if (!p.waves && !F32) consider(6, time(fwd[6], 128, 128, true, odd ? 1.1f : 1.f));
         }
         if (best == 0) return launch_rows<DT, ST, HALF, 1, 1, GRAD>(p, st);
         if (best == 1) return launch_rows<DT, ST, HALF, 1, 2, GRAD>(p, st);
@@ -1062,7 +1063,7 @@ static hipError_t launch_typed(const W4Params& p, hipStream_t st) {
         if (most >= 4) consider(1, time(grad[1], 64, 16, false, 1.f));
         if (p.N > 16) {
             if (most == 8) consider(2, time(grad[2], 128, 32, true, 1.f));
-            consider(3, time(grad[3], 128, tiled_cols, true, 1.f));
+            if (!p.waves) consider(3, time(grad[3], 128, tiled_cols, true, 1.f));
         }
         if (best == 0) return launch_rows<DT, ST, HALF, 1, 2, GRAD>(p, st);
         if (best == 1) return launch_rows<DT, ST, HALF, 1, 4, GRAD>(p, st);

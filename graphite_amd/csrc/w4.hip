@@ -123,7 +123,7 @@ static hipError_t w4_launch(const W4Params& p, int dt, int scale_type, bool grad
 }
 
 static int w4_run(gr_ctx* ctx, const gr_w4* w, const char* who, bool grad, const void* x, int dt, int64_t N, int64_t ldx, const void* gate,
-                  int64_t ldg, int relu, void* y, int64_t ldy, hipStream_t st) {
+                  int64_t ldg, int relu, void* y, int64_t ldy, int waves, hipStream_t st) {
     if (!w) return gr_fail(ctx, GR_EINVAL, "%s: null layer", who);
     if (w->ctx != ctx) return gr_fail(ctx, GR_ESTATE, "%s: the layer belongs to another context", who);
     if (!dt_ok(dt)) return gr_fail(ctx, GR_EINVAL, "%s: unknown element type %d", who, dt);
@@ -144,7 +144,7 @@ static int w4_run(gr_ctx* ctx, const gr_w4* w, const char* who, bool grad, const
     p.chunks = (grad ? w->Mp : w->Kp) / W4_CHUNK;
     p.gsteps = w->group / 32;
     p.x = x; p.y = y; p.bias = w->bias; p.gate = gate;
-    p.N = N; p.ldx = ldx; p.ldy = ldy; p.ldg = ldg; p.relu = relu;
+    p.N = N; p.ldx = ldx; p.ldy = ldy; p.ldg = ldg; p.relu = relu; p.waves = waves;
     const double fl = 2.0 * (double)N * w->M * w->K;
     const double by = (double)w->M * w->K / 2 + (double)w->M * w->G * (dt_size(w->st) + (w->has_zeros ? 1 : 0)) + (double)N * (w->M + w->K) * es;
     ProfScope ps(ctx, grad ? "k_w4_grad" : "k_w4_forward", st, fl, by);
@@ -157,11 +157,24 @@ extern "C" int gr_linear_w4(gr_ctx* ctx, const gr_w4* w, const void* x, int dtyp
                             int64_t ldy, void* stream) {
     if (!ctx) return GR_EINVAL;
     GR_HIP(ctx, hipSetDevice(ctx->device));
-    return w4_run(ctx, w, "gr_linear_w4", false, x, dtype, N, ldx, nullptr, 0, relu, y, ldy, (hipStream_t)stream);
+    return w4_run(ctx, w, "gr_linear_w4", false, x, dtype, N, ldx, nullptr, 0, relu, y, ldy, 0, (hipStream_t)stream);
 }
 extern "C" int gr_linear_w4_input_grad(gr_ctx* ctx, const gr_w4* w, const void* grad_y, int dtype, int64_t N, int64_t ldgy,
                                        const void* gate, int64_t ldgate, void* grad_x, int64_t ldgx, void* stream) {
     if (!ctx) return GR_EINVAL;
     GR_HIP(ctx, hipSetDevice(ctx->device));
-    return w4_run(ctx, w, "gr_linear_w4_input_grad", true, grad_y, dtype, N, ldgy, gate, ldgate, 0, grad_x, ldgx, (hipStream_t)stream);
+    return w4_run(ctx, w, "gr_linear_w4_input_grad", true, grad_y, dtype, N, ldgy, gate, ldgate, 0, grad_x, ldgx, 0, (hipStream_t)stream);
+}
+
+// Waves of a model's layers: the few-row kernels add in an order that only their number decides (a wave's chunks in turn, then
+// the waves), so with a fixed one an image's logits and gradient are the same bits in every chunk, like the float layers'.
+// GTSRBNet, groups of 64, us: 1 image 314 with 4 waves, 313 with 8 and 313 with the layers' own choice; 8192 images 13548,
+// 13635 and 13370 (the tiled kernel, whose order is another).
+constexpr int W4_MODEL_WAVES = 4;
+int w4_model_forward(gr_ctx* ctx, const gr_w4* w, const float* x, int64_t N, int64_t ldx, int relu, float* y, int64_t ldy, hipStream_t st) {
+    return w4_run(ctx, w, "gr_linear_w4", false, x, GR_DT_F32, N, ldx, nullptr, 0, relu, y, ldy, W4_MODEL_WAVES, st);
+}
+int w4_model_input_grad(gr_ctx* ctx, const gr_w4* w, const float* grad_y, int64_t N, int64_t ldgy, const float* gate, int64_t ldgate,
+                        float* grad_x, int64_t ldgx, hipStream_t st) {
+    return w4_run(ctx, w, "gr_linear_w4_input_grad", true, grad_y, GR_DT_F32, N, ldgy, gate, ldgate, 0, grad_x, ldgx, W4_MODEL_WAVES, st);
 }

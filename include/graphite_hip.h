@@ -227,8 +227,9 @@ int gr_model_input_grad_topk(gr_ctx* ctx, gr_model* m, const float* x, int N, co
 /* Runs a linear layer of the model on 4-bit weights (gr_w4_create, in_features in PyTorch's order): GTSRBNet layer 0 = fc5_1,
  * 1 = fc6_1, 2 = fc7_1; WideResNet and BagNet layer 0 = fc.  Forward, predict, gr_tr_hits and the input gradients follow it;
  * the activations stay float32 (GTSRBNet: GR_EINVAL together with GR_PREC_BF16).  w must have been created with input_grad if
- * gradients are taken, belongs to the caller and must outlive its use; NULL puts the float layer back.  The logits of an image
- * may differ in their last bits between batch sizes. */
+ * gradients are taken, belongs to the caller and must outlive its use; NULL puts the float layer back.  An image's logits and
+ * its gradient for a label do not depend on the batch or chunk it is in (gr_linear_w4 by itself: last bits may, other kernels
+ * serve other sizes); neither do they, nor the soft-target gradient, depend on how a call is cut into chunks. */
 struct gr_w4;
 int gr_model_set_linear_w4(gr_model* m, int layer, const struct gr_w4* w);
 

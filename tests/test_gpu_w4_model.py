@@ -253,3 +253,76 @@ def test_refusals():
                 TeacherTop(top.index.repeat(2, 1), top.value.repeat(2, 1), None, 1.0)):
         with pytest.raises(E):
             m.hip_model.input_grad_topk(x, bad)
+
+
+@pytest.mark.parametrize("group", [32, 64, 96, 256])
+def test_an_image_gets_the_same_bits_in_every_batch(group):
+    """Chunk size, workspace limit and rank count decide which images pass a layer together; results do not follow them."""
+    sd = synth.gtsrb_state_dict(readout="toy3")
+    m = models.GTSRBNet().load_state_dict(sd).quantize_linear(sd, group)
+    x = torch.from_numpy(synth.synth_images("w4-batches", 1030)).cuda()
+    top = teacher_top(m.forward(x[:1]), 5, 2.0)
+    logits, labels = m.forward(x), m.hip_model.predict_dev(x)
+    grads, soft = m.hip_model.input_grad(x, 3)[1], m.hip_model.input_grad_topk(x, top)[1]
+    for a, b in ((0, 1), (3, 20), (100, 137), (0, 640), (300, 1024), (1024, 1030)):
+        assert torch.equal(m.forward(x[a:b]), logits[a:b]) and torch.equal(m.hip_model.predict_dev(x[a:b]), labels[a:b])
+        assert torch.equal(m.hip_model.input_grad(x[a:b], 3)[1], grads[a:b])
+        if a % 4 == 0:                                  # the loss sums a row of 43 logits from its first 16-byte border on
+            assert torch.equal(m.hip_model.input_grad_topk(x[a:b], top)[1], soft[a:b])
+    try:
+        for limit in (64 << 20, 150 << 20):             # 80 images a chunk and more
+            _hip.set_workspace_limit(limit)
+            assert torch.equal(m.forward(x), logits) and torch.equal(m.hip_model.input_grad(x, 3)[1], grads)
+            assert torch.equal(m.hip_model.input_grad_topk(x, top)[1], soft)
+    finally:
+        _hip.set_workspace_limit(8 << 30)
+
+
+def test_heads_of_the_other_models_in_every_batch():
+    from graphite_amd.patchguard.patchguard_predict import PatchGuard
+    sd = synth.wrn_state_dict("wrn-w4", depth=10, widen=2, num_classes=10)
+    x = torch.from_numpy(synth.synth_images("wrn-batches", 700, 0.0, 1.0)).cuda()
+    m = models.WideResNet(depth=10, num_classes=10, widen_factor=2).load_state_dict(sd).quantize_linear(sd, 32)
+    logits = m.forward(x)
+    for a, b in ((0, 1), (3, 20), (100, 641)):
+        assert torch.equal(m.forward(x[a:b]), logits[a:b])
+    sd = synth.bagnet_state_dict()
+    key = "fc" if "fc.weight" in sd else "module.fc"
+    q, s, z = quantize(sd[key + ".weight"], 64)
+    p = PatchGuard(sd)
+    p.hip_model.set_linear_w4(0, LinearW4(q, s, z, bias=torch.as_tensor(sd[key + ".bias"]), group=64))
+    x = torch.from_numpy(synth.synth_images("bag-batches", 24)).cuda()
+    local = p.local_logits(x)
+    for a, b in ((0, 1), (3, 20)):
+        assert torch.equal(p.local_logits(x[a:b]), local[a:b])
+
+
+def test_hits_do_not_follow_the_chunk():
+    a, _, _ = _pair(64)
+    c = gtsrb_case(num_xforms=60)
+    masks, thetas = gtsrb_candidates(c, 12)
+    lib, ctx = _hip.load_library(), _hip.ctx()
+    want = None
+    try:
+        for chunk in (8192, 64, 200, 641):
+            assert lib.gr_ctx_set_chunk(ctx, chunk) == 0
+            hits, preds = engine.tr_hits(a, c["vic"], masks, thetas, c["tab"], 27, return_preds=True)
+            want = (hits, preds) if want is None else want
+            assert torch.equal(hits, want[0]) and torch.equal(preds, want[1])
+    finally:
+        lib.gr_ctx_set_chunk(ctx, 8192)
+
+
+def test_gradient_chunks_of_a_few_images():
+    """WideResNet-34-10 keeps 17 MB an image: 64 MiB hold three, and a chunk is four."""
+    sd = synth.wrn_state_dict()
+    m = models.WideResNet(num_classes=10).load_state_dict(sd).quantize_linear(sd, 64)
+    x = torch.from_numpy(synth.synth_images("wrn-chunks", 11, 0.0, 1.0)).cuda()
+    top = teacher_top(m.forward(x[:1]), 3, 1.0)
+    want = m.hip_model.input_grad(x, 3)[1], m.hip_model.input_grad_topk(x, top)[1]
+    try:
+        _hip.set_workspace_limit(64 << 20)
+        got = m.hip_model.input_grad(x, 3)[1], m.hip_model.input_grad_topk(x, top)[1]
+    finally:
+        _hip.set_workspace_limit(8 << 30)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and bool(want[0].any()) and bool(want[1].any())
