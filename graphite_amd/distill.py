@@ -9,6 +9,7 @@ engine.eot_gradient(..., teacher=top) takes the whitebox step on it.
 from collections import namedtuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _hip
 
@@ -47,6 +48,9 @@ def topk_distill(logits, index, value, tau=1.0, teacher_lse=None, grad_loss=None
     if value.device != dev or vt is None:
         raise _hip.GraphiteHipError(f"value must be a float32, bfloat16 or float16 tensor on {dev}")
     index, value = index.contiguous(), value.contiguous()
+    graph = z.requires_grad and torch.is_grad_enabled()
+    if graph and grad_out is not None and grad_out.untyped_storage().data_ptr() == z.untyped_storage().data_ptr():
+        raise _hip.GraphiteHipError("grad_out in the place of logits that require a gradient: pass logits.detach()")
     lse_p = gl_p = grad_p = None
     if teacher_lse is not None:
         teacher_lse = _vector(teacher_lse, "teacher_lse", rows, dev)
@@ -66,7 +70,25 @@ def topk_distill(logits, index, value, tau=1.0, teacher_lse=None, grad_loss=None
         grad_p = grad.data_ptr()
     _hip.op_call("gr_distill_topk", dev, z.data_ptr(), _hip.DTYPES[dt], n, v, ldz, index.data_ptr(), value.data_ptr(), vt, k,
                  0 if rows == 1 else k, lse_p, float(tau), gl_p, loss.data_ptr(), grad_p, ldg)
+    if graph:
+        loss = _Loss.apply(z, loss, index, value, float(tau), teacher_lse)
     return loss, grad
+
+
+class _Loss(torch.autograd.Function):
+    """The loss of `z`, already computed, as a function of it."""
+
+    @staticmethod
+    def forward(ctx, z, loss, index, value, tau, lse):
+        ctx.save_for_backward(z, index, value, lse)
+        ctx.tau = tau
+        return loss.view_as(loss)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_loss):
+        z, index, value, lse = ctx.saved_tensors
+        return topk_distill(z, index, value, ctx.tau, lse, grad_loss)[1], None, None, None, None, None
 
 
 def _vector(t, name, size, dev):

@@ -6,12 +6,14 @@
     gx = layer.input_grad(gy)                                 # d loss / d x, for the whitebox loops
 
 float32, bfloat16 and float16 activations; every product is exact, every sum float32, the result is rounded once.
+Where x requires a gradient, y takes part in torch.autograd (once differentiable; the weights and the bias are frozen).
 models.GTSRBNet.set_linear_w4 runs a victim's fully connected layers this way.
 """
 import ctypes as C
 
 import numpy as np
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _hip
 
@@ -58,6 +60,25 @@ def dequantize(q, scales, zeros=None, group=64, in_features=None):
     grp = torch.arange(k, device=q.device) // group
     z = 8.0 if zeros is None else zeros.float()[:, grp]
     return (codes - z) * scales.float()[:, grp]
+
+
+class _Forward(torch.autograd.Function):
+    """layer.forward(x, relu) of [rows, in], differentiable w.r.t. x (gr_linear_w4_input_grad)."""
+
+    @staticmethod
+    def forward(ctx, x, layer, relu):
+        y = layer.forward(x, relu=relu)
+        ctx.layer, ctx.relu = layer, relu
+        if relu:
+            ctx.save_for_backward(y)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_y):
+        if ctx.relu:
+            grad_y = grad_y.masked_fill(ctx.saved_tensors[0] <= 0, 0)
+        return ctx.layer.input_grad(grad_y), None, None
 
 
 class LinearW4:
@@ -116,13 +137,19 @@ class LinearW4:
 
     def forward(self, x, relu=False, out=None):
         """x [..., in] -> [..., out] of x's type on the current stream; relu clamps negative results to 0.  Rows of x may be
-        any distance apart.  out: optional result tensor [rows, out], which must not overlap x."""
+        any distance apart.  out: optional result tensor [rows, out], which must not overlap x and takes no part in
+        torch.autograd."""
         lead = None
         if x.dim() != 2:
             lead = x.shape[:-1]
             x = x.reshape(-1, x.shape[-1])
         x, ldx = _hip.float_rows(x, "x", self.device, self.in_features)
         n, m = x.shape[0], self.out_features
+        if x.requires_grad and torch.is_grad_enabled():
+            if out is not None:
+                raise _hip.GraphiteHipError("out= takes no part in torch.autograd, and x requires a gradient: pass x.detach(), or no out")
+            y = _Forward.apply(x, self, relu)
+            return y if lead is None else y.view(*lead, m)
         if out is None:
             y, ldy = x.new_empty((n, m)), m
         else:
@@ -134,7 +161,8 @@ class LinearW4:
 
     def input_grad(self, grad_y, gate=None, out=None):
         """grad_y [..., out] -> d loss / d x [..., in] of its type; 0 where gate <= 0 (gate: the rectified activation the
-        layer read, shape of the result).  A ReLU of this layer is the caller's to apply to grad_y.  out: as forward's."""
+        layer read, shape of the result).  A ReLU of this layer is the caller's to apply to grad_y.  out: as forward's.
+        The result is a plain tensor: it carries no graph, whatever grad_y requires."""
         lead = None
         if grad_y.dim() != 2:
             lead = grad_y.shape[:-1]

@@ -294,3 +294,46 @@ def test_rows_past_one_launch():
     assert torch.equal(loss.view(-1, t), want_l.expand(n // t, t)) and torch.equal(grad.view(-1, t, 2), want_g.expand(n // t, t, 2))
     del loss, grad
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rest", [False, True], ids=["closed", "open"])
+def test_loss_takes_part_in_autograd(rest, dtype):
+    """backward() of the loss gives the gradient of the explicit form for the same grad_loss, bit for bit."""
+    z, top, gl = _inputs(6, 300, 5, dtype, 41)
+    lse = top.lse if rest else None
+    want_l, want_g = topk_distill(z, top.index, top.value, 1.0, lse, gl)
+    leaf = z.clone().requires_grad_(True)
+    loss, grad = topk_distill(leaf, top.index, top.value, 1.0, lse, gl)
+    assert loss.requires_grad and not grad.requires_grad and torch.equal(loss, want_l) and torch.equal(grad, want_g)
+    (loss * gl).sum().backward()
+    assert leaf.grad.dtype == dtype and torch.equal(leaf.grad, want_g)
+    leaf.grad = None
+    (2.0 * leaf).backward(topk_distill(2.0 * leaf.detach(), top.index, top.value, 1.0, lse)[1])     # the explicit form stays
+    assert leaf.grad.shape == z.shape
+    leaf.grad = None
+    topk_distill(leaf, top.index, top.value, 1.0, lse, want_grad=False)[0].sum().backward()           # expanded gradient
+    assert torch.equal(leaf.grad, topk_distill(z, top.index, top.value, 1.0, lse)[1])
+    with torch.no_grad():
+        assert not topk_distill(leaf, top.index, top.value, 1.0, lse)[0].requires_grad
+    with pytest.raises(_hip.GraphiteHipError):
+        topk_distill(leaf, top.index, top.value, 1.0, lse, grad_out=leaf)
+    out = torch.empty_like(z)
+    loss, grad = topk_distill(leaf, top.index, top.value, 1.0, lse, gl, grad_out=out)
+    assert grad is out and loss.requires_grad and torch.equal(out, want_g)
+    (g,) = torch.autograd.grad(loss.sum(), leaf, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
+def test_layer_and_loss_train_an_input_together():
+    """The whitebox step written with torch.autograd: the 4-bit layer's logits, the loss, the gradient at the input; against the
+    explicit chain."""
+    from graphite_amd.linear_w4 import LinearW4, quantize
+    g = torch.Generator().manual_seed(43)
+    layer = LinearW4(*quantize(torch.randn((43, 256), generator=g) / 16, 64), group=64)
+    x = torch.randn((20, 256), generator=g).cuda().requires_grad_(True)
+    top = teacher_top(torch.randn((1, 43), generator=g).cuda() * 2, 5, 2.0)
+    topk_distill(layer.forward(x), top.index, top.value, 2.0, top.lse)[0].mean().backward()
+    _, gz = topk_distill(layer.forward(x.detach()), top.index, top.value, 2.0, top.lse, torch.full((20,), 1 / 20, device="cuda"))
+    assert torch.equal(x.grad, layer.input_grad(gz))

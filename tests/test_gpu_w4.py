@@ -488,3 +488,64 @@ def test_float32_gradient_extremes(n, k, m):
     gx = layer.input_grad(torch.from_numpy(gy).float().cuda()).double().cpu().numpy()
     ref = torch.from_numpy(gy).float().double().numpy() @ w
     assert (np.abs(gx - ref) <= 2.0 ** -21 * np.abs(ref)).all()
+
+
+@pytest.mark.parametrize("relu", [False, True], ids=["linear", "relu"])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+def test_forward_takes_part_in_autograd(dtype, relu):
+    """backward() gives what input_grad gives for the same grad_y, bit for bit, and the formula's gradient."""
+    layer, w, b = _layer(75, 200, 64, bias=True, seed=21)
+    g = torch.Generator().manual_seed(22)
+    x = torch.randn((2, 9, 200), generator=g).to("cuda", dtype).requires_grad_(True)
+    gy = torch.randn((2, 9, 75), generator=g).to("cuda", dtype)
+    y = layer.forward(x, relu=relu)
+    assert y.requires_grad and torch.equal(y, layer.forward(x.detach(), relu=relu))
+    y.backward(gy)
+    want = gy.masked_fill(y.detach() <= 0, 0) if relu else gy
+    assert x.grad.dtype == dtype and torch.equal(x.grad, layer.input_grad(want))
+    gd = want.double().cpu().numpy().reshape(18, 75)
+    ref = R.input_grad(gd, w)
+    _check(x.grad.reshape(18, 200), ref, _tol(ref, np.abs(gd) @ np.abs(w), 75 + 64, dtype, 2.0 ** -15))
+    # broadcast gradients (sum), transposed and shared inputs, twice through the same layer
+    a = torch.randn((200, 5), generator=g).cuda().requires_grad_(True)
+    (layer.forward(a.t()).sum() + layer.forward(a.t()).mul(2.0).sum()).backward()
+    ref = 3.0 * np.repeat(w.sum(0)[:, None], 5, 1)
+    _check(a.grad, ref, 3.0 * np.abs(w).sum(0)[:, None] * (140 * 2.0 ** -23 + 2.0 ** -22) + 1e-30)
+    with torch.no_grad():
+        assert not layer.forward(x).requires_grad
+    with pytest.raises(_hip.GraphiteHipError):
+        layer.forward(a.t(), out=torch.empty(5, 75, device="cuda"))
+    one = _layer(75, 200, 64, seed=21)[0]
+    (gx,) = torch.autograd.grad(one.forward(a.t()).sum(), a, create_graph=True)
+    with pytest.raises(RuntimeError):
+        gx.sum().backward()
+    no = LinearW4(torch.zeros((4, 16), dtype=torch.uint8), torch.ones((4, 1)), group=32, input_grad=False)
+    with pytest.raises(_hip.GraphiteHipError):
+        no.forward(torch.ones((2, 32), device="cuda", requires_grad=True)).sum().backward()
+
+
+def test_autograd_in_a_captured_graph():
+    layer, _, _ = _layer(200, 330, 64, bias=True, seed=23)
+    x, gy = torch.zeros((40, 330), device="cuda"), torch.randn((40, 200), device="cuda")
+
+    def step():
+        leaf = x.detach().requires_grad_(True)
+        y = layer.forward(leaf, relu=True)
+        return y.detach(), torch.autograd.grad(y, leaf, gy)[0]
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, gx = step()
+    for i in range(3):
+        x.copy_(torch.randn((40, 330), generator=torch.Generator().manual_seed(i)))
+        graph.replay()
+        torch.cuda.synchronize()
+        yw, gw = step()
+        assert torch.equal(y, yw) and torch.equal(gx, gw)
+        torch.cuda.synchronize()
