@@ -322,7 +322,10 @@ int gr_linear_w4_input_grad(gr_ctx* ctx, const gr_w4* w, const void* grad_y, int
  *               tau (P q_i - target_i) with P = sum p + p_rest, p_rest counted only where the loss counts it
  * grad may be z itself (ldg == ldz) but must not overlap it otherwise.  A row without slots (all -1; closed: also all values -inf) has loss 0 and gradient 0.
  * An index outside [-1, V) makes its row's loss and gradient NaN.  1 <= k <= 1024; 1e-6 <= tau <= 1e6; V <= 2^20 in the
- * open form.  No workspace, no allocation: the call can be captured into a HIP graph.  Results do not vary between runs. */
+ * open form.  No workspace, no allocation: the call can be captured into a HIP graph.  Results do not vary between runs.
+ * Probabilities are float32: the gradient, a difference of two, is off by up to about 2^-21 tau |grad_loss| (P q_i + target_i);
+ * the loss by 2^-21 tau^2, above tau = 4 by that times |q_rest - p_rest| in the open form and by a rounding of the result in the
+ * closed form with every class named. */
 int gr_distill_topk(gr_ctx* ctx, const void* z, int dtype, int64_t N, int V, int64_t ldz, const int64_t* index, const void* value,
                     int value_type, int k, int64_t ld_top, const float* teacher_lse, float tau, const float* grad_loss, float* loss,
                     void* grad, int64_t ldg, void* stream);

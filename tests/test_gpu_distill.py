@@ -337,3 +337,27 @@ def test_layer_and_loss_train_an_input_together():
     topk_distill(layer.forward(x), top.index, top.value, 2.0, top.lse)[0].mean().backward()
     _, gz = topk_distill(layer.forward(x.detach()), top.index, top.value, 2.0, top.lse, torch.full((20,), 1 / 20, device="cuda"))
     assert torch.equal(x.grad, layer.input_grad(gz))
+
+
+@pytest.mark.parametrize("tau", [1.0, 20.0, 100.0, 1000.0, 1e4])
+@pytest.mark.parametrize("k", [5, 43], ids=["open", "all-named"])
+def test_loss_at_high_temperatures(k, tau):
+    """Student and teacher nearly alike: the loss is tau^2 times a sum that all but cancels.  Open form: with one or no unnamed
+    logit a lane, Sr is off by e = (3 U + 4 + 8) 2^-24 (three roundings of u, exp2's last bits, adding), the loss by
+    tau^2 |q_rest - p_rest| e and, second order, tau^2 e^2; closed with every class named it holds no float sum.  Both: 64-bit
+    arithmetic, tau^2 2^-46, and the rounding of the result."""
+    z, top, _ = _inputs(8, 43, k, F32, 51, tau=tau)
+    lse = top.lse if k < 43 else None
+    loss, _ = topk_distill(z, top.index, top.value, tau, lse)
+    zd, idx, val = z.double().cpu().numpy(), top.index.cpu().numpy(), top.value.double().cpu().numpy()
+    ref, _ = R.distill(zd, idx, val, tau, None if lse is None else lse.double().cpu().numpy())
+    tol = tau * tau * 2.0 ** -46 + np.abs(ref) * 2.0 ** -23
+    if lse is not None:
+        q = np.exp(zd / tau)
+        q /= q.sum(1, keepdims=True)
+        q_rest = 1 - np.take_along_axis(q, idx, 1).sum(1)
+        p_rest = 1 - np.exp(val / tau - lse.double().cpu().numpy()[:, None]).sum(1)
+        e = (3 * np.ptp(zd, axis=1) / tau + 12) * 2.0 ** -24
+        tol = tol + tau * tau * (np.abs(q_rest - p_rest) * e + e * e)
+    err = np.abs(loss.double().cpu().numpy() - ref)
+    assert (err <= tol).all(), (err / tol).max()
