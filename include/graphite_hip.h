@@ -294,7 +294,9 @@ int gr_w4_create(gr_ctx* ctx, const uint8_t* q, int64_t ldq, const void* scales,
                  gr_w4** out);
 void gr_w4_destroy(gr_w4* w);
 /* x [N][in_features] (rows ldx elements apart) -> y [N][out_features] (rows ldy apart), both of type dtype; relu != 0 clamps
- * negative results to 0.  The products are exact and the sums float32; the result is rounded to dtype once.  Elements
+ * negative results to 0.  The products are exact and the sums float32; the result is rounded to dtype once.  A group's sum of
+ * x times integers precedes its scale: it must stay finite (certain for |x| < 2^124 / min(group, in_features)); float32 x below
+ * 2^-109 counts to within 2^-132.  Elements
  * between rows are not touched.  x and y must not overlap.  No workspace, no allocation, no synchronisation: the call can be
  * captured into a HIP graph. */
 int gr_linear_w4(gr_ctx* ctx, const gr_w4* w, const void* x, int dtype, int64_t N, int64_t ldx, int relu, void* y, int64_t ldy,
