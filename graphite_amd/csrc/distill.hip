@@ -139,7 +139,7 @@ __device__ __forceinline__ float kd_block(float x, float none, float* slots, OP 
 
 // One workgroup per row.  VPT 16-byte vectors per thread of the row stay in registers between the pass that finds its maximum,
 // the one that sums and the one that writes the gradient, so the row is read from memory once; what does not fit (BIG) is read
-// again, mostly from the caches.  Bound by memory: 4096 x 32768 bf16 125 us = 4.3 TB/s, a copy of that size takes 100 us.
+// again, mostly from the caches.  Bound by memory: 4096 x 32768 bf16 120 us = 4.5 TB/s, a copy of that size takes 100 us.
 // The teacher's few classes are the first wave's work.
 // LDS (dynamic): p [k] double | z [k] float | i [k] int | bits, one per class (OPEN), bit 32 = the first aligned element.
 template <int DT, int NT, int VPT, bool BIG, bool OPEN>
@@ -425,7 +425,7 @@ hipError_t launch(const KdParams& p, hipStream_t st) {
     // (8192 rows of 2048 bf16: 64 threads 27 us, 256 45, 1024 146); long ones need loads in flight, and few rows many waves
     // (4096 rows of 32768 bf16: 256 threads with the row in registers 125 us, 1024 130; 1 row of 131072 f32: 1024 threads 26 us,
     // 256 66).  Rows beyond 64 KB are read twice rather than held by 1024 threads x 16 vectors, which spill (4096 x 32768 f32
-    // 238 us against 260, 515 x 100003 135 against 143).
+    // 238 us against 260, 515 x 100003 135 against 143); 512 such workgroups run at a time, so the last 3 of 515 rows run alone.
     if (nv <= 64 * 4) return launch1<DT, 64, 4, false, OPEN>(p, st);
     if (nv <= 256 * 4) return launch1<DT, 256, 4, false, OPEN>(p, st);
     if (nv <= 1024 * 4) return p.N >= 512 ? launch1<DT, 256, 16, false, OPEN>(p, st) : launch1<DT, 1024, 4, false, OPEN>(p, st);

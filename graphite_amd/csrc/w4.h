@@ -289,7 +289,7 @@ __device__ __forceinline__ void w4_put(const W4Params& p, w4_f32x4 sum, const fl
 // Forward: GS = groups of a chunk (1, 2 or 4; 4 also where a border falls on any step).
 // One row is bound by the weights' bytes: the matrix unit pads it to 16 rows for nothing, and what costs is turning nibbles
 // into operands, 2.5 VALU instructions a weight.  8192 -> 8192 bf16, g = 128, one row: 10.8 us = 3.2 TB/s of weights (a copy
-// reaches 4.7).  2048 -> 1024 f32, 100 rows: 8.1 us a call (its latency: two chunks a wave, then the join, in which a thread
+// reaches 4.7).  2048 -> 1024 f32, 100 rows: 8.2 us a call (its latency: one chunk a wave, then the join, in which a thread
 // adds and stores four outputs at once; one output a thread took 9.2).
 // ---------------------------------------------------------------------------------------------
 constexpr int w4_rows_waves(int nt) { return nt > 1 ? 8 : 16; }            // the most a workgroup may have
@@ -484,8 +484,8 @@ __global__ __launch_bounds__(w4_rows_waves(NT) * 64) void k_w4_rows(W4Params p) 
 // [16 bytes], the order the packed weights already have), so every LDS access is 64 lanes x 16 consecutive bytes.
 // Three LDS buffers, one barrier per stage: while a stage is multiplied, the next one's first operands are already read and
 // the one after is written, from registers that global memory filled a stage earlier.
-// Measured (4096 -> 4096, 4096 rows, bf16): 160 us = 857 TFLOP/s, a library product of that size 1220; its gradient at 2048 rows
-// 131 us = 525 (1050 of matrix work, two pieces); 8192 x 2048 -> 1024 f32 118 us = 291 (873 of matrix work; the f32 matrix
+// Measured (4096 -> 4096, 4096 rows, bf16): 159 us = 865 TFLOP/s, a library product of that size 1220; its gradient at 2048 rows
+// 131 us = 526 (1050 of matrix work, two pieces); 8192 x 2048 -> 1024 f32 118 us = 292 (875 of matrix work; the f32 matrix
 // unit's peak is 157).  Nothing is saturated: the matrix unit is busy 35 % of the cycles (gradient 40), VALU issue takes 46,
 // LDS 35; two waves a SIMD, in step through the barrier, overlap them only in part.  Tried and slower, against 192 us at the
 // time (the code for groups of 32 still in the same kernel, which spilled for it):  4-wave workgroups of 128 x 128 (251 us),
@@ -1004,9 +1004,10 @@ static hipError_t launch_typed(const W4Params& p, hipStream_t st) {
     // and something for each output.  In microseconds:  out * workgroups / 256 + chunk * chunks * rounds, where rounds is
     //   max(1, workgroups / (256 * more))            for small workgroups, several of which share a CU,
     //   1 + more * (ceil(workgroups / 256) - 1)      for large ones (LDS), one a CU.
-    // The numbers are fitted to the variants' times at 900 sizes (17 to 8192 rows, 33 to 8192 on both sides, every group).  The
-    // variant with the least estimate takes 3 to 6 % longer than the fastest one (geometric mean); limits on the number of
-    // output tiles took 6 to 13 % and up to 3.3 times as long.
+    // The numbers are fitted to the variants' times at 900 sizes (17 to 8192 rows, 33 to 8192 on both sides, every group).  At 340
+    // others (profiles/lowbit_variant_times.csv) the variant with the least estimate takes 2 to 6 % longer than the fastest one
+    // (geometric mean by direction and type; at most 37 %); limits on the number of output tiles took 6 to 13 % and up to 3.3
+    // times as long.
     // Small tiles carry short contractions and few rows, the tiled kernel large products (us, in the order of `fwd`):  bf16,
     // 320 rows 96 -> 6528  10.7 8.4 9.3 10.3 14.4 11.5;  f32, 384 rows 7680 -> 2848  -, -, 169 122 217 184;  bf16, 2464 rows
     // 3648 -> 2048  -, -, 159 110 138 81.  The tiled kernel's half tile: 2048 rows 4096 -> 4096 bf16, groups of 128  116 (whole
