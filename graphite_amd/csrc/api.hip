@@ -514,7 +514,8 @@ static int model_input_grad(gr_ctx* ctx, gr_model* m, const char* who, const flo
     const int ncls = gr_model_num_classes(m);
     // the pass keeps every activation: ~0.8 MB per image for GTSRBNet, ~17 MB for WideResNet-34-10
     int64_t cap = (int64_t)(ctx->ws_limit / (net_grad_workspace_bytes(m, 64) / 64 + 1));
-    cap = cap < 4 ? 4 : cap > 1024 ? 1024 : cap / 4 * 4;    // by fours: a row of logits keeps its place within 16 bytes in every chunk
+    if (cap < 1) cap = 1;
+    if (cap > 1024) cap = 1024;
     int chunk = N < cap ? N : (int)cap;
     if (chunk <= 0) return GR_OK;
     int rc = gr_ws_reserve(ctx, net_grad_workspace_bytes(m, chunk), stream);
@@ -528,6 +529,7 @@ static int model_input_grad(gr_ctx* ctx, gr_model* m, const char* who, const flo
             part.value += n0 * part.ld_top;
             if (part.lse && part.ld_top) part.lse += n0;
             if (part.loss) part.loss += n0;
+            part.shift = (int)((int64_t)n0 * ncls % 4);
         }
         if ((rc = net_input_grad(ctx, m, x + (size_t)n0 * 3072, nb, target, soft ? &part : nullptr, logits ? logits + (size_t)n0 * ncls : nullptr,
                                  grad_x + (size_t)n0 * 3072, ctx->ws, ctx->ws_bytes, st))) return rc;
@@ -544,7 +546,7 @@ extern "C" int gr_model_input_grad_topk(gr_ctx* ctx, gr_model* m, const float* x
                                         void* stream) {
     NEED_CTX();
     if (!index || !value || k < 1 || (ld_top != 0 && ld_top < k)) return gr_fail(ctx, GR_EINVAL, "gr_model_input_grad_topk: bad arguments");
-    const NetSoftTarget soft = {index, value, teacher_lse, k, ld_top, tau, loss};
+    const NetSoftTarget soft = {index, value, teacher_lse, k, ld_top, tau, loss, 0};
     return model_input_grad(ctx, m, "gr_model_input_grad_topk", x, N, 0, &soft, logits, grad_x, stream);
 }
 

@@ -132,7 +132,9 @@ int net_pg_local(gr_ctx*, gr_model*, const float* x_chw, int N, float* local, ch
 int net_pg_out_size(const gr_model*);
 // d loss / d x_n: forward with every activation kept, then the transposed layers.  loss = CE(logits_n, target), or the
 // distillation loss of `soft` (gr_distill_topk) when that is given
-struct NetSoftTarget { const int64_t* index; const float* value; const float* lse; int k; int64_t ld_top; float tau; float* loss; };
+// shift: where the chunk's first row of logits would lie within 16 bytes in the whole batch's (floats): the loss sums a row from its
+// first 16-byte border on, and its bits are not to depend on the chunk
+struct NetSoftTarget { const int64_t* index; const float* value; const float* lse; int k; int64_t ld_top; float tau; float* loss; int shift; };
 int net_input_grad(gr_ctx*, gr_model*, const float* x_chw, int N, int target, const NetSoftTarget* soft, float* logits_or_null,
                    float* grad_x, char* ws, size_t ws_bytes, hipStream_t);
 size_t net_grad_workspace_bytes(const gr_model*, int N);

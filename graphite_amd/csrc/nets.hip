@@ -1289,7 +1289,7 @@ int net_input_grad(gr_ctx* ctx, gr_model* m, const float* x, int N, int target, 
     hipLaunchKernelGGL(k_maxpool2_fwd, blocks((size_t)N * 2048), dim3(256), 0, st, a42, N, 8, 8, 128, p4);
     if ((rc = gtsrb_fc(ctx, m, 0, p4, N, f5, gA, st))) return rc;
     if ((rc = gtsrb_fc(ctx, m, 1, f5, N, f6, nullptr, st))) return rc;
-    float* lgp = logits_out ? logits_out : lg;
+    float* lgp = logits_out ? logits_out : lg + (soft ? soft->shift : 0);      // lg has 64 floats an image, more than classes
     if ((rc = gtsrb_fc(ctx, m, 2, f6, N, lgp, nullptr, st))) return rc;
     // ---- backward: every transposed layer gates its output with the ReLU of the activation it produces the gradient of ----
     if ((rc = logit_grad(ctx, m, lgp, N, target, soft, g64, st))) return rc;
@@ -1435,7 +1435,7 @@ static int wrn_input_grad(gr_ctx* ctx, gr_model* m, const float* x, int N, int t
     }
     const int C3 = m->ch[3], P = H * H;
     hipLaunchKernelGGL(k_avgpool, blocks((size_t)N * C3), dim3(256), 0, st, OF, N, P, C3, pooled);
-    float* lgp = logits_out ? logits_out : lg;
+    float* lgp = logits_out ? logits_out : lg + (soft ? soft->shift : 0);      // lg has 64 floats an image, more than classes
     if (m->w4[0]) { if ((rc = w4_model_forward(ctx, m->w4[0], pooled, N, C3, 0, lgp, m->ncls, st))) return rc; }
     else if ((rc = run_conv(ctx, m->wfc, pooled, N, 1, 1, nullptr, nullptr, lgp, nullptr, false, false, st))) return rc;
     // ---- backward ----

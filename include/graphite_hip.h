@@ -296,16 +296,15 @@ void gr_w4_destroy(gr_w4* w);
 /* x [N][in_features] (rows ldx elements apart) -> y [N][out_features] (rows ldy apart), both of type dtype; relu != 0 clamps
  * negative results to 0.  The products are exact and the sums float32; the result is rounded to dtype once.  A group's sum of
  * x times integers precedes its scale: it must stay finite (certain for |x| < 2^124 / min(group, in_features)); float32 x below
- * 2^-109 counts to within 2^-132.  Elements
- * between rows are not touched.  x and y must not overlap.  No workspace, no allocation, no synchronisation: the call can be
- * captured into a HIP graph. */
+ * 2^-109 counts to within 2^-132.  Elements between rows are not touched.  x and y must not overlap.  No workspace, no
+ * allocation, no synchronisation: the call can be captured into a HIP graph. */
 int gr_linear_w4(gr_ctx* ctx, const gr_w4* w, const void* x, int dtype, int64_t N, int64_t ldx, int relu, void* y, int64_t ldy,
                  void* stream);
 /* grad_x[n,k] = sum_m grad_y[n,m] * (q[m,k] - z[m,k / group]) * s[m,k / group], 0 where gate[n,k] <= 0 (gate: the rectified
  * activation the layer read, same type as grad_x, rows ldgate apart; NULL = no gate).  The layer's own ReLU, if it had one,
  * is the caller's to apply to grad_y.  Same promises as gr_linear_w4, but for the products: each is off by at most
- * 1.5 * 2^-23 of itself in float32 and 2^-15 in the 16-bit types, with either sign; a row of grad_y with an infinity or NaN gives a row of infinities and NaNs.  The weights are frozen: no
- * gradient is formed for them. */
+ * 1.5 * 2^-23 of itself in float32 and 2^-15 in the 16-bit types, with either sign; a row of grad_y with an infinity or NaN
+ * gives a row of infinities and NaNs.  The weights are frozen: no gradient is formed for them. */
 int gr_linear_w4_input_grad(gr_ctx* ctx, const gr_w4* w, const void* grad_y, int dtype, int64_t N, int64_t ldgy, const void* gate,
                             int64_t ldgate, void* grad_x, int64_t ldgx, void* stream);
 

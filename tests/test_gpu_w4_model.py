@@ -314,15 +314,25 @@ def test_hits_do_not_follow_the_chunk():
 
 
 def test_gradient_chunks_of_a_few_images():
-    """WideResNet-34-10 keeps 17 MB an image: 64 MiB hold three, and a chunk is four."""
+    """WideResNet-34-10 keeps 17 MB an image: 64 MiB hold three, whose rows of logits lie elsewhere within 16 bytes than the whole
+    batch's; also where the caller asks for no logits."""
     sd = synth.wrn_state_dict()
     m = models.WideResNet(num_classes=10).load_state_dict(sd).quantize_linear(sd, 64)
     x = torch.from_numpy(synth.synth_images("wrn-chunks", 11, 0.0, 1.0)).cuda()
     top = teacher_top(m.forward(x[:1]), 3, 1.0)
-    want = m.hip_model.input_grad(x, 3)[1], m.hip_model.input_grad_topk(x, top)[1]
+    h, p = m.hip_model, _hip._p
+
+    def no_logits():
+        loss, gx = torch.empty(11, device="cuda"), torch.empty_like(x)
+        assert _hip.load_library().gr_model_input_grad_topk(_hip.ctx(), h._h, p(x), 11, p(top.index), p(top.value), 3, 0, p(top.lse), 1.0,
+                                                            p(loss), None, p(gx), _hip._stream()) == 0
+        return loss, gx
+
+    want = h.input_grad(x, 3)[1], *h.input_grad_topk(x, top)[1:], *no_logits()
+    assert torch.equal(want[1], want[4]) and torch.equal(want[2], want[3]) and bool(want[0].any()) and bool(want[1].any())
     try:
         _hip.set_workspace_limit(64 << 20)
-        got = m.hip_model.input_grad(x, 3)[1], m.hip_model.input_grad_topk(x, top)[1]
+        got = h.input_grad(x, 3)[1], *h.input_grad_topk(x, top)[1:], *no_logits()
     finally:
         _hip.set_workspace_limit(8 << 30)
-    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and bool(want[0].any()) and bool(want[1].any())
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
